@@ -168,6 +168,95 @@ int turt_permute4(turt_ctx* ctx, const float* inp, float* out, const int* inShap
 int turt_adamw(turt_ctx* ctx, const float* grad, float* param, float* m, float* v, size_t n, float lr, float b1,
                float b2, float eps, float wd, float bc1, float bc2);                                 /* :783-788 */
 
+/* ------------------------------------------------- paged cache, rules on logits
+ * Serving several sequences at once: their keys and values live in pages of a common pool, and the
+ * logits of their next tokens follow per-request rules.  No reference counterpart (the reference
+ * samples one sequence and keeps no cache).
+ *
+ * A paged cache holds, for kv head h and position j of sequence b, the head_dim elements at
+ *   page_table[b * max_pages + j / page_size] * page_stride + h * head_stride
+ *     + (j % page_size) * slot_stride
+ * of `k` and of `v` (strides in elements; the elements of one position are contiguous).  Zero
+ * strides mean the packed layout [n_pages][n_kv_head][page_size][head_dim].  Sequences may share
+ * pages that are only read.  Table entries of pages that no call reads or writes may hold any
+ * value.  head_dim is even, 2 .. 256. */
+#define TURT_CACHE_F32 0
+#define TURT_CACHE_F16 1
+#define TURT_CACHE_BF16 2
+typedef struct turt_paged_kv {
+  void* k;                    /* device */
+  void* v;                    /* device, same type and layout */
+  const uint32_t* page_table; /* device [batch][max_pages] */
+  const uint32_t* lens;       /* device [batch]: positions of each sequence, new ones included; 0 = idle */
+  size_t page_stride, head_stride, slot_stride;
+  int dtype;                  /* TURT_CACHE_* */
+  int n_pages, page_size, n_kv_head, head_dim;
+  int batch, max_pages;
+} turt_paged_kv;
+
+/* Appends `rows` new positions: row i holds the n_kv_head * head_dim keys k[i * k_stride ...] and
+ * values v[i * v_stride ...] of one position.  Rows start[b] .. start[b+1] - 1 (start: device
+ * uint32[batch + 1], not decreasing) are the last positions of sequence b, so its first new row
+ * goes to position lens[b] - (start[b+1] - start[b]).  Without `start` (NULL) rows = batch and row
+ * b is the last position of sequence b; idle sequences take none.  Rows before start[0] or from
+ * start[batch] on are skipped.
+ * The first rot_dim (even, 0 .. head_dim; 0 = no rotation) elements of each key head are rotated
+ * in interleaved pairs by position * base^(-2m / rot_dim), as turt_rope does, with the angle in
+ * double precision; keys and values are rounded once, to nearest even, to the cache's type.
+ * q (may be NULL) holds n_head query heads per row, which are rotated alike into q_out (q_out = q
+ * with equal strides rotates in place; rows that are skipped are left as they were).
+ * A position that the page table does not reach, a page number >= n_pages, or more new rows than
+ * lens[b] raise TURT_ERR_RANGE at the next synchronization, and those rows are skipped.  No two
+ * rows of a call may go to the same cache position through a shared page. */
+int turt_paged_append(turt_ctx* ctx, const turt_paged_kv* kv, const float* k, size_t k_stride, const float* v,
+                      size_t v_stride, const float* q, size_t q_stride, float* q_out, size_t q_out_stride, int n_head,
+                      const uint32_t* start, int rows, int rot_dim, float base);
+
+/* Attention of one new token per sequence over its cached positions: for query head a of sequence
+ * b, which reads kv head a / (n_head / n_kv_head),
+ *   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  s_j = scale * q . k_j,  m = max_j s_j
+ * over j in [max(0, lens[b] - window), lens[b]) (window 0 = all).  q[b * q_stride ...] and
+ * out[b * out_stride ...] hold n_head * head_dim floats per sequence, rotated already.  lse (may be
+ * NULL; [batch][n_head]) receives m + ln(sum exp(s_j - m)).  A sequence without positions, or
+ * whose scores are all -infinity, gives zeros and -infinity.  Products and sums are in fp32 whatever the cache's type, in an order that
+ * depends on the sizes only: equal calls give equal bits.
+ * The length of each sequence is read on the device, so a captured call may be replayed with other
+ * lengths, page tables and contents.  `workspace` (device, 16-byte aligned, at least
+ * turt_paged_attention_workspace bytes for the same sizes) must be zero before its first use
+ * (turt_buffer zeroes) and is left ready for the next call, of the same or other sizes; calls that
+ * may overlap, replayed graphs among them, each need one of their own.
+ * A page number >= n_pages or a length beyond max_pages * page_size raises TURT_ERR_RANGE at the
+ * next synchronization; the positions on such a page are left out, and such a sequence gives zeros. */
+int turt_paged_attention_workspace(const turt_paged_kv* kv, int n_head, size_t* bytes);
+int turt_paged_attention(turt_ctx* ctx, const turt_paged_kv* kv, const float* q, size_t q_stride, float* out,
+                         size_t out_stride, float* lse, int n_head, float scale, int window, void* workspace,
+                         size_t workspace_bytes);
+
+/* Rules on the logits of `rows` next tokens (all pointers device; each group may be NULL):
+ * row r knows the ids tokens[token_start[r] .. token_start[r+1]), of which those from
+ * generated_start[r] on (NULL: none) were generated and the others belong to the prompt. */
+typedef struct turt_logit_rules {
+  const uint32_t* tokens;
+  const uint32_t* token_start;     /* [rows + 1] */
+  const uint32_t* generated_start; /* [rows], index into tokens */
+  const float* repetition;         /* [rows], > 0: ids of the prompt or generated: x > 0 ? x / r : x * r */
+  const float* frequency;          /* [rows]: x -= f * (times generated) */
+  const float* presence;           /* [rows]: x -= p where generated at all */
+  const uint32_t* bias_ids;        /* strictly increasing within a row */
+  const float* bias;               /* added after the penalties */
+  const uint32_t* bias_start;      /* [rows + 1] */
+  const uint32_t* mask;            /* [n_masks][ceil(vocab / 32)]: bit id % 32 of word id / 32 = 0: -infinity */
+  const uint32_t* mask_row;        /* [rows]: mask of each row, 0xFFFFFFFF = none; NULL: row r has mask r */
+  int n_masks;
+} turt_logit_rules;
+/* out[r * out_ld + id] = the rules, in the order of the fields above, of logits[r * ld + id] for
+ * id < vocab; out = logits with equal pitches works in place.  A masked entry is -infinity
+ * whatever the logit was; a mask without a set bit leaves nothing.  Ids >= vocab, bias ids that do
+ * not increase and masks >= n_masks raise TURT_ERR_RANGE at the next synchronization; the ids are
+ * skipped, such a mask counts as none. */
+int turt_logit_rules_apply(turt_ctx* ctx, const float* logits, size_t ld, float* out, size_t out_ld, int rows,
+                           int vocab, const turt_logit_rules* rules);
+
 /* ----------------------------------------------------- host-array matmul
  * GpuCompute.matmul / bmm, src/infer/webgpu/gpu.ts:66-141, and Backend.matmul,
  * src/infer/backend.ts:11-16 / gpu-backend.ts:45-55: host arrays in, host array out. */

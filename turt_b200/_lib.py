@@ -42,6 +42,23 @@ class TurtConfig(C.Structure):
                 ("n_embd", C.c_int), ("arch", C.c_int), ("hidden", C.c_int)]
 
 
+CACHE_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+class TurtPagedKv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_table", C.c_void_p), ("lens", C.c_void_p),
+                ("page_stride", C.c_size_t), ("head_stride", C.c_size_t), ("slot_stride", C.c_size_t),
+                ("dtype", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv_head", C.c_int),
+                ("head_dim", C.c_int), ("batch", C.c_int), ("max_pages", C.c_int)]
+
+
+class TurtLogitRules(C.Structure):
+    _fields_ = [("tokens", C.c_void_p), ("token_start", C.c_void_p), ("generated_start", C.c_void_p),
+                ("repetition", C.c_void_p), ("frequency", C.c_void_p), ("presence", C.c_void_p),
+                ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("bias_start", C.c_void_p),
+                ("mask", C.c_void_p), ("mask_row", C.c_void_p), ("n_masks", C.c_int)]
+
+
 _SCALARS = {"int": C.c_int, "size_t": C.c_size_t, "float": C.c_float, "double": C.c_double,
             "uint16_t": C.c_uint16, "uint32_t": C.c_uint32, "uint64_t": C.c_uint64}
 

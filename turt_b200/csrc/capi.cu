@@ -31,7 +31,9 @@ int ctx_check_flags(turt_ctx* ctx) {
       return ERR_TIMEOUT;
     }
     if (h[FLAG_RANGE]) {
-      set_error("token or target id out of range [0, vocab)");
+      set_error(h[FLAG_RANGE] == RANGE_PAGE   ? "page number or position out of range of the paged cache"
+                : h[FLAG_RANGE] == RANGE_RULE ? "token, bias id or mask of a logit rule out of range"
+                                              : "token or target id out of range [0, vocab)");
       return ERR_RANGE;
     }
     set_error("non-finite loss or gradient norm");

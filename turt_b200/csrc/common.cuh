@@ -79,10 +79,16 @@ int smem_attr_per_device(std::atomic<uint64_t>& done, K kfn, int bytes) {
 
 // Device-side error flags (one int array per context, see DeviceFlags).
 enum FlagIndex : int {
-  FLAG_RANGE = 0,    // bad token / target id seen
+  FLAG_RANGE = 0,    // bad id seen (RANGE_* says of what)
   FLAG_TIMEOUT = 1,  // bounded wait expired (value = site code)
   FLAG_NONFINITE = 2,
   FLAG_COUNT = 4,
+};
+// Values of FLAG_RANGE.
+enum RangeKind : int {
+  RANGE_TOKEN = 1,  // token / target id
+  RANGE_PAGE = 2,   // page number or position of a paged cache
+  RANGE_RULE = 3,   // id or mask of a logit rule
 };
 
 // ------------------------------------------------------------- device utils

@@ -188,6 +188,28 @@ class GpuEngine:
     def adamw(self, grad, param, m, v, n, lr, b1, b2, eps, wd, bc1, bc2):
         check(self.L.turt_adamw(self.h, grad, param, m, v, n, lr, b1, b2, eps, wd, bc1, bc2))
 
+    # ------------------------------------------- paged cache, rules on logits (no reference counterpart)
+    def pagedAppend(self, kv, k, kStride, v, vStride, rows, start=None, q=None, qStride=0, qOut=None, qOutStride=0,
+                    nHead=0, rotDim=0, base=10000.0):
+        check(self.L.turt_paged_append(self.h, C.byref(kv), k, kStride, v, vStride, q, qStride, qOut, qOutStride, nHead,
+                                       start, rows, rotDim, base))
+
+    def pagedAttentionWorkspace(self, kv, nHead) -> int:
+        """Bytes of workspace that pagedAttention needs for these sizes (zeroed before its first use)."""
+        n = C.c_size_t()
+        check(self.L.turt_paged_attention_workspace(C.byref(kv), nHead, C.byref(n)))
+        return n.value
+
+    def pagedAttention(self, kv, q, qStride, out, outStride, nHead, workspace, workspaceBytes, scale=None, window=0,
+                       lse=None):
+        """scale None = 1 / sqrt(head_dim)."""
+        check(self.L.turt_paged_attention(self.h, C.byref(kv), q, qStride, out, outStride, lse, nHead,
+                                          1 / math.sqrt(kv.head_dim) if scale is None else scale, window, workspace,
+                                          workspaceBytes))
+
+    def logitRules(self, logits, ld, out, outLd, rows, vocab, rules):
+        check(self.L.turt_logit_rules_apply(self.h, logits, ld, out, outLd, rows, vocab, C.byref(rules)))
+
 
 class GpuTensor:
     """GPU-resident autograd tensor (autograd.ts:817-1210)."""

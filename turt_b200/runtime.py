@@ -10,7 +10,8 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import ARCH_GPT2, ARCH_MODERN, TurtConfig, check, f32, lib, ptr, u32
+from ._lib import (ARCH_GPT2, ARCH_MODERN, CACHE_TYPES, TurtConfig, TurtLogitRules, TurtPagedKv, check, f32, lib, ptr,
+                   u32)
 
 
 class Context:
@@ -79,6 +80,24 @@ class Context:
 def make_config(vocab_size, block_size, n_layer, n_head, n_embd, arch="modern", hidden=0) -> TurtConfig:
     return TurtConfig(vocab_size, block_size, n_layer, n_head, n_embd,
                       ARCH_MODERN if arch == "modern" else ARCH_GPT2, hidden)
+
+
+def make_paged_kv(k, v, page_table, lens, dtype, n_pages, page_size, n_kv_head, head_dim, batch, max_pages,
+                  page_stride=0, head_stride=0, slot_stride=0) -> TurtPagedKv:
+    """Descriptor of a paged key / value cache over device pointers (dtype "f32", "f16" or "bf16");
+    zero strides mean the packed layout [n_pages][n_kv_head][page_size][head_dim]."""
+    if dtype not in CACHE_TYPES:
+        raise ValueError(f"cache type must be one of {list(CACHE_TYPES)}, got {dtype!r}")
+    return TurtPagedKv(k, v, page_table, lens, page_stride, head_stride, slot_stride, CACHE_TYPES[dtype], n_pages,
+                       page_size, n_kv_head, head_dim, batch, max_pages)
+
+
+def make_logit_rules(tokens=None, token_start=None, generated_start=None, repetition=None, frequency=None,
+                     presence=None, bias_ids=None, bias=None, bias_start=None, mask=None, mask_row=None,
+                     n_masks=0) -> TurtLogitRules:
+    """Rules on logits (penalties, biases, masks) over device pointers; None leaves a rule out."""
+    return TurtLogitRules(tokens, token_start, generated_start, repetition, frequency, presence, bias_ids, bias,
+                          bias_start, mask, mask_row, n_masks)
 
 
 class Model:
