@@ -1,5 +1,5 @@
-// paged.cu -- the paged key / value cache: appending new positions with their rotation, and the
-// attention of one new token per sequence over its pages.
+// paged.cu -- the paged key / value cache: its descriptor, and appending new positions with their
+// rotation (reading it: paged_attend.cu).
 //
 // The single-sequence decode step (decode.cu) keeps one contiguous fp32 cache with as many key
 // heads as query heads.  Here many sequences share a pool of pages (so none reserves its longest
@@ -57,8 +57,6 @@ int paged_layout(const turt_paged_kv* kv, PagedLayout* out) {
 }
 
 namespace {
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // --------------------------------------------------------------------------------- append
 //
@@ -207,90 +205,6 @@ int append_launch(cudaStream_t st, const AppendArgs& a, bool vec) {
   return OK;
 }
 
-// ------------------------------------------------------------------------------ attention
-
-struct AttendArgs {
-  PagedLayout kv;
-  const void *kc, *vc;
-  const float* q;
-  float *out, *lse;
-  size_t qs, os;
-  int heads, window;
-  float scale;
-  int* flags;
-};
-
-constexpr int kAttendWarps = 8;
-
-// One block per (query head, sequence): warps take every 8th position, lanes every 32nd element,
-// each warp keeping its running max, sum and unnormalised output; joined through shared memory.
-template <typename T>
-__global__ void __launch_bounds__(kAttendWarps * 32) k_paged_attend(const __grid_constant__ AttendArgs a) {
-  __shared__ float sm[kAttendWarps], sl[kAttendWarps], so[kAttendWarps][256];
-  const PagedLayout& kv = a.kv;
-  const int h = blockIdx.x, b = blockIdx.y, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = h / (a.heads / kv.kv_heads), dim = kv.dim;
-  uint32_t n = kv.lens[b];
-  if (n > kv.max_pages * kv.page_size) {
-    if (threadIdx.x == 0) atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
-    n = 0;
-  }
-  const uint32_t j0 = a.window > 0 && n > (uint32_t)a.window ? n - a.window : 0;
-  float q[8], o[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const int d = lane + 32 * i;
-    q[i] = d < dim ? a.q[(size_t)b * a.qs + (size_t)h * dim + d] : 0.f;
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (uint32_t j = j0 + w; j < n; j += kAttendWarps) {
-    const uint32_t page = kv.table[(size_t)b * kv.max_pages + j / kv.page_size];
-    if (page >= kv.n_pages) {
-      if (lane == 0) atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
-      continue;
-    }
-    const size_t off =
-        (size_t)page * kv.page_stride + (size_t)hk * kv.head_stride + (size_t)(j % kv.page_size) * kv.slot_stride;
-    const T* kr = (const T*)a.kc + off;
-    const T* vr = (const T*)a.vc + off;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (lane + 32 * i < dim) s += q[i] * to_f32(kr[lane + 32 * i]);
-    s = warp_sum(s) * a.scale;
-    const float top = fmaxf(m, s), f = top == -INFINITY ? 1.f : expf(m - top);
-    const float p = s == -INFINITY ? 0.f : expf(s - top);
-    m = top;
-    l = l * f + p;
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (lane + 32 * i < dim) o[i] = o[i] * f + p * to_f32(vr[lane + 32 * i]);
-  }
-  if (lane == 0) {
-    sm[w] = m;
-    sl[w] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; i++) so[w][lane + 32 * i] = o[i];
-  __syncthreads();
-  float top = sm[0], sum = 0.f;
-  for (int i = 1; i < kAttendWarps; i++) top = fmaxf(top, sm[i]);
-  float f[kAttendWarps];
-#pragma unroll
-  for (int i = 0; i < kAttendWarps; i++) {
-    f[i] = sm[i] == -INFINITY && sl[i] == 0.f ? 0.f : expf(sm[i] - top);  // a warp without positions
-    sum += f[i] * sl[i];
-  }
-  for (int d = threadIdx.x; d < dim; d += blockDim.x) {
-    float y = 0.f;
-#pragma unroll
-    for (int i = 0; i < kAttendWarps; i++) y += f[i] * so[i][d];
-    a.out[(size_t)b * a.os + (size_t)h * dim + d] = top == -INFINITY && sum == 0.f ? 0.f : y / sum;
-  }
-  if (a.lse && threadIdx.x == 0) a.lse[(size_t)b * a.heads + h] = top == -INFINITY && sum == 0.f ? -INFINITY : top + logf(sum);
-}
-
 }  // namespace
 }  // namespace turt
 
@@ -342,49 +256,4 @@ extern "C" int turt_paged_append(turt_ctx* ctx, const turt_paged_kv* kv, const f
   if (kv->dtype == TURT_CACHE_F32) return append_launch<float>(ctx->stream, a, vec);
   if (kv->dtype == TURT_CACHE_F16) return append_launch<__half>(ctx->stream, a, vec);
   return append_launch<__nv_bfloat16>(ctx->stream, a, vec);
-}
-
-extern "C" int turt_paged_attention_workspace(const turt_paged_kv* kv, int n_head, size_t* bytes) {
-  PagedLayout p;
-  RC(paged_layout(kv, &p));
-  TURT_REQUIRE(bytes, "paged_attention_workspace: null bytes");
-  TURT_REQUIRE(n_head > 0 && n_head % kv->n_kv_head == 0, "paged_attention: n_head must be a multiple of n_kv_head");
-  *bytes = 16;
-  return OK;
-}
-
-extern "C" int turt_paged_attention(turt_ctx* ctx, const turt_paged_kv* kv, const float* q, size_t q_stride, float* out,
-                                    size_t out_stride, float* lse, int n_head, float scale, int window, void* workspace,
-                                    size_t workspace_bytes) {
-  AttendArgs a;
-  size_t need = 0;
-  RC(paged_layout(kv, &a.kv));
-  RC(turt_paged_attention_workspace(kv, n_head, &need));
-  const size_t wide = (size_t)n_head * kv->head_dim;
-  TURT_REQUIRE(kv->batch == 0 || (q && out), "paged_attention: null pointer");
-  TURT_REQUIRE(kv->batch <= 1 || (q_stride >= wide && out_stride >= wide),
-               "paged_attention: row strides below the row width");
-  TURT_REQUIRE(window >= 0, "paged_attention: negative window");
-  TURT_REQUIRE(isfinite(scale), "paged_attention: scale must be finite");
-  TURT_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)lse) % 4 == 0, "paged_attention: misaligned pointer");
-  TURT_REQUIRE(workspace && workspace_bytes >= need && aligned16(workspace),
-               "paged_attention: workspace missing, misaligned or smaller than turt_paged_attention_workspace says");
-  TURT_REQUIRE(ctx, "null context");
-  TURT_CHECK_CUDA(cudaSetDevice(ctx->device));
-  if (kv->batch == 0) return OK;
-  TURT_REQUIRE(kv->batch <= 65535, "paged_attention: at most 65535 sequences");
-  a.kc = kv->k, a.vc = kv->v;
-  a.q = q, a.out = out, a.lse = lse;
-  a.qs = q_stride, a.os = out_stride;
-  a.heads = n_head, a.window = window, a.scale = scale;
-  a.flags = ctx->flags;
-  const dim3 grid(n_head, kv->batch);
-  if (kv->dtype == TURT_CACHE_F32)
-    k_paged_attend<float><<<grid, kAttendWarps * 32, 0, ctx->stream>>>(a);
-  else if (kv->dtype == TURT_CACHE_F16)
-    k_paged_attend<__half><<<grid, kAttendWarps * 32, 0, ctx->stream>>>(a);
-  else
-    k_paged_attend<__nv_bfloat16><<<grid, kAttendWarps * 32, 0, ctx->stream>>>(a);
-  TURT_LAUNCH_CHECK();
-  return OK;
 }

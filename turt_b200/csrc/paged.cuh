@@ -21,6 +21,7 @@ struct PagedLayout {
 // Checks a descriptor and resolves its strides (0 = packed [page][head][slot][dim]).
 int paged_layout(const turt_paged_kv* kv, PagedLayout* out);
 
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline size_t cache_type_size(int dtype) { return dtype == TURT_CACHE_F32 ? 4 : 2; }
 
 __device__ __forceinline__ float to_f32(float x) { return x; }

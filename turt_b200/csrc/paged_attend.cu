@@ -1,0 +1,1034 @@
+// paged_attend.cu -- attention of one new token per sequence over a paged key / value cache.
+//
+//   s_j = scale q . k_j,  out = sum_j 2^(s_j' - m) v_j / sum_j 2^(s_j' - m),  s' = s log2(e)
+//
+// Every cached key and value is read once and used by the heads of its group only, so the bound is
+// the memory bandwidth.  The positions of all sequences and key heads form one line of tiles, cut
+// into equal stretches, one per warp of a grid that fills the GPU once: ragged lengths, one long
+// sequence and many short ones load all warps alike, whatever the lengths are (they are read on the
+// device).  A warp streams its tiles through a ring of shared memory of its own with 16-byte
+// asynchronous copies, so nothing but its own copies holds it up; it runs the online softmax of its
+// stretch in registers.  A part of a sequence that a warp did not see whole is joined with its
+// neighbours': first inside the block, then by the last block to arrive, always in the order of
+// positions.
+#include <math.h>
+
+#include <algorithm>
+
+#include "ctx.cuh"
+#include "paged.cuh"
+
+namespace turt {
+namespace {
+
+constexpr int kMaxBlocks = 512;           // counters and partial results in the workspace
+constexpr int kPrefix = 1024;             // entries of the tile prefix held in shared memory
+constexpr int kGroup = 8;                 // heads of a group that a warp treats at once, at most
+constexpr float kLazy = 8.0f;             // the running max moves when it is this far behind (log2)
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;  // no cached position behind this row of a tile
+
+struct AttendArgs {
+  PagedLayout kv;
+  const void *kc, *vc;
+  const float* q;
+  float *out, *lse;
+  size_t qs, os;
+  int heads, group, window;
+  int chunks;        // parts of a group: ceil(group / heads per part)
+  int part;          // heads per part
+  float scale;       // times log2(e)
+  uint32_t div_mul;  // position / page_size = position * div_mul >> div_shift (positions < 2^31)
+  int div_shift;
+  int min_tiles;     // tiles per warp, at least
+  uint32_t* counters;
+  float* partial;
+  int* flags;
+};
+
+__device__ __forceinline__ uint32_t page_of(const AttendArgs& a, uint32_t j) {
+  return (uint32_t)(((uint64_t)j * a.div_mul) >> a.div_shift);
+}
+
+__device__ __forceinline__ float exp2_of(float s, float m) { return exp2f(s - (m == -INFINITY ? 0.f : m)); }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The positions that sequence b attends to: [first, n) in tiles [t0, t1) of KT.
+struct Seq {
+  uint32_t n, first, t0, t1;
+};
+template <int KT>
+__device__ __forceinline__ Seq seq_of(const AttendArgs& a, int b) {
+  Seq s;
+  s.n = a.kv.lens[b];
+  if (s.n > a.kv.max_pages * a.kv.page_size) s.n = 0;  // flagged where the batch is scanned
+  s.first = a.window > 0 && s.n > (uint32_t)a.window ? s.n - a.window : 0;
+  s.t0 = s.first / KT;
+  s.t1 = (s.n + KT - 1) / KT;
+  return s;
+}
+
+// A place on the line of tiles (sequence, part of a head group, tile).
+template <int KT>
+struct Walk {
+  Seq s;
+  int b, hc;
+  uint32_t t;
+  __device__ void next(const AttendArgs& a, int hcs) {
+    if (++t < s.t1) return;
+    t = s.t0;
+    if (++hc < hcs) return;
+    hc = 0;
+    do {
+      if (++b >= a.kv.batch) return;
+      s = seq_of<KT>(a, b);
+    } while (s.n == 0);
+    t = s.t0;
+  }
+};
+
+// A result of part of a sequence: per head m (log2), l and dim unnormalised outputs.
+__device__ __forceinline__ int rec_floats(const AttendArgs& a) { return a.part * (a.kv.dim + 2); }
+
+__device__ __forceinline__ float weight_of(float m, float l, float top) {
+  return m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
+}
+
+__device__ __forceinline__ void store_out(const AttendArgs& a, int b, int head, int d, float o, float l) {
+  a.out[(size_t)b * a.os + (size_t)head * a.kv.dim + d] = l == 0.f ? 0.f : o / l;
+}
+__device__ __forceinline__ void store_lse(const AttendArgs& a, int b, int head, float m, float l) {
+  if (a.lse) a.lse[(size_t)b * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// One warp, any layout, head by head: positions [j0, j1) of sequence b into rec (one record of
+// a.part heads).  Lanes take every 32nd element.  The formula as it stands: also what a stretch
+// with infinities or NaN falls back to.
+template <typename T>
+__device__ __noinline__ void attend_plain(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
+  const PagedLayout& kv = a.kv;
+  const int lane = threadIdx.x & 31, dim = kv.dim;
+  const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * a.part;
+  for (int g = 0; g < a.part; g++) {
+    float q[8], o[8], m = -INFINITY, l = 0.f;
+    const float* qh = a.q + (size_t)b * a.qs + (size_t)(hk * a.group + g0 + g) * dim;
+    const bool head = g0 + g < a.group;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      q[i] = head && lane + 32 * i < dim ? qh[lane + 32 * i] * a.scale : 0.f;
+      o[i] = 0.f;
+    }
+    for (uint32_t j = j0; head && j < j1; j++) {
+      const uint32_t pg = page_of(a, j), id = kv.table[(size_t)b * kv.max_pages + pg];
+      if (id >= kv.n_pages) continue;  // flagged where the tile was opened
+      const size_t off = (size_t)id * kv.page_stride + (size_t)hk * kv.head_stride +
+                         (size_t)(j - pg * kv.page_size) * kv.slot_stride;
+      const T *kr = (const T*)a.kc + off, *vr = (const T*)a.vc + off;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (lane + 32 * i < dim) s += q[i] * to_f32(kr[lane + 32 * i]);
+      s = warp_sum(s);
+      const float top = fmaxf(m, s), f = top == -INFINITY ? 1.f : exp2f(m - top);
+      const float p = s == -INFINITY ? 0.f : exp2f(s - top);
+      m = top;
+      l = l * f + p;
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (lane + 32 * i < dim) o[i] = o[i] * f + p * to_f32(vr[lane + 32 * i]);
+    }
+    float* r = rec + g * (dim + 2);
+    if (lane == 0) {
+      r[0] = m;
+      r[1] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (lane + 32 * i < dim) r[2 + lane + 32 * i] = o[i];
+  }
+  __syncwarp();
+}
+
+// Paths: how a warp treats the tiles of its stretch.
+//   issue(stage, row, ok)   starts the copies of a tile; lane r < KT holds row r's place in 16-byte units
+//   begin / tile / finish   the softmax of one part of a sequence; finish leaves its record in rec
+// ------------------------------------------------------------------------------- any layout
+template <typename T>
+struct PathPlain {
+  static constexpr int KT = 16, WARPS = 8, STAGES = 1, STAGE_BYTES = 0;
+  static constexpr bool RING = false;
+  __device__ void setup(const AttendArgs&, char*) {}
+  __device__ void begin(const AttendArgs&, int, int) {}
+  __device__ void issue(const AttendArgs&, char*, int, uint32_t) {}
+  __device__ void tile(const AttendArgs&, char*, uint32_t) {}
+  __device__ void finish(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
+    attend_plain<T>(a, b, hc, j0, j1, rec);
+  }
+};
+
+// -------------------------------------------------------------- 16-bit caches: tensor cores
+//
+// A tile is 16 positions.  S = Q K^T and O += P V are m16n8k16 products with the heads of the group
+// (8 at most) as rows.  Only the cache is 16-bit: q and the weights p are fp32 and go in as a sum of
+// 16-bit parts, one part in rows 0-7 and the next in rows 8-15 of the same product, so the unused
+// half of the rows buys the precision: fp16 takes two parts (22 bits; q scaled per head to [1, 2)
+// by a power of two), bf16 three (24 bits; the third in a product of its own).  The thread that
+// holds row r also holds row r + 8, so the parts of a score and of an output meet in one register,
+// and the scores are where the next product wants p.  Each tile's product is added to the running
+// output in fp32 outside the tensor cores, whose own accumulation truncates.
+// Infinities and NaN break the parts (0 * inf): a stretch that ends in a non-finite result is done
+// again by attend_plain.
+template <typename T>
+struct Half2;
+template <>
+struct Half2<__half> {
+  static constexpr bool THREE = false;
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <>
+struct Half2<__nv_bfloat16> {
+  static constexpr bool THREE = true;
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// KD: steps of 16 elements that cover head_dim (a multiple of 8).
+template <typename T, int KD>
+struct PathMma {
+  using H = Half2<T>;
+  static constexpr int KT = 16, WARPS = 8, UNIT = 8;
+  static constexpr bool RING = true;
+  // rows an odd number of 16-byte units apart: the eight rows of an ldmatrix fall into different banks
+  static constexpr int PITCH = (2 * KD + 1) * 16;
+  static constexpr int STAGE_BYTES = 2 * KT * PITCH;
+  static constexpr int STAGES = KD >= 6 ? 2 : KD >= 4 ? 3 : 4;
+
+  uint32_t qa[KD][4], qb[H::THREE ? KD : 1][2];
+  float acc[2 * KD][2], m, l, unscale;
+  uint32_t units, div;  // 16-byte units of a row; e / units = e * div >> 16 for e < 256
+
+  __device__ void setup(const AttendArgs& a, char* ring) {
+    units = a.kv.dim / 8;
+    div = (65536 + units - 1) / units;
+    if (units < 2 * KD)  // the copies leave the padding of a row as it is: zero
+      for (int s = 0; s < STAGES; s++)
+        for (int e = (threadIdx.x & 31) * 16; e < STAGE_BYTES; e += 512)
+          *reinterpret_cast<uint4*>(ring + s * (STAGE_BYTES + 16) + e) = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  }
+
+  __device__ void begin(const AttendArgs& a, int b, int hc) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = (lane & 3) * 2, dim = a.kv.dim;
+    const int hk = hc / a.chunks, g = (hc - hk * a.chunks) * a.part + r;
+    const bool head = r < a.part && g < a.group;
+    const float* q = a.q + (size_t)b * a.qs + (size_t)(hk * a.group + (head ? g : 0)) * dim;
+    float x[KD][4], top = 0.f;
+#pragma unroll
+    for (int k = 0; k < KD; k++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int d = k * 16 + (i >> 1) * 8 + c + (i & 1);
+        x[k][i] = head && d < dim ? q[d] * a.scale : 0.f;
+        top = fmaxf(top, fabsf(x[k][i]));
+      }
+    float up = 1.f;
+    unscale = 1.f;
+    if constexpr (!H::THREE) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t ex = __float_as_uint(top) >> 23;
+      if (ex >= 1 && ex < 253) {
+        up = __uint_as_float((254 - ex) << 23);
+        unscale = __uint_as_float(ex << 23);
+      } else if (ex >= 253) {
+        unscale = NAN;  // leads to attend_plain
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < KD; k++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        float u = x[k][2 * i] * up, v = x[k][2 * i + 1] * up;
+        const uint32_t p0 = H::pack(u, v);
+        const float2 f0 = H::unpack(p0);
+        u -= f0.x, v -= f0.y;
+        const uint32_t p1 = H::pack(u, v);
+        qa[k][2 * i] = p0;
+        qa[k][2 * i + 1] = p1;
+        if constexpr (H::THREE) {
+          const float2 f1 = H::unpack(p1);
+          qb[k][i] = H::pack(u - f1.x, v - f1.y);
+        }
+      }
+#pragma unroll
+    for (int j = 0; j < 2 * KD; j++) acc[j][0] = acc[j][1] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+  }
+
+  __device__ void issue(const AttendArgs& a, char* st, int lane, uint32_t row) {
+    const uint32_t dst = smem_u32(st);
+#pragma unroll
+    for (int i = 0; i < KD; i++) {
+      const uint32_t e = i * 32 + lane, rr = (e * div) >> 16, u = e - rr * units;
+      const uint32_t at = __shfl_sync(0xffffffffu, row, rr & 15);
+      if (rr < KT) {
+        const size_t off = at == kNoRow ? 0 : ((size_t)at << 4) + u * 16;
+        const uint32_t n = at == kNoRow ? 0 : 16;
+        cp_async16(dst + rr * PITCH + u * 16, (const char*)a.kc + off, n);
+        cp_async16(dst + (KT + rr) * PITCH + u * 16, (const char*)a.vc + off, n);
+      }
+    }
+  }
+
+  __device__ void tile(const AttendArgs&, char* st, uint32_t ok) {
+    const int lane = threadIdx.x & 31, c = (lane & 3) * 2;
+    const uint32_t ks = smem_u32(st) + ((lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
+    const uint32_t vs = smem_u32(st) + (KT + (lane & 15)) * PITCH + (lane >> 4) * 16;
+    float d0[2][4] = {}, d1[2][4] = {};
+#pragma unroll
+    for (int k = 0; k < KD; k++) {
+      uint32_t b[4];
+      ldmatrix4(b, ks + k * 32);
+      H::mma(d0[0], qa[k], b[0], b[1]);
+      H::mma(d0[1], qa[k], b[2], b[3]);
+      if constexpr (H::THREE) {
+        const uint32_t low[4] = {qb[k][0], 0, qb[k][1], 0};
+        H::mma(d1[0], low, b[0], b[1]);
+        H::mma(d1[1], low, b[2], b[3]);
+      }
+    }
+    float s[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; n++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const float x = d0[n][i] + (d0[n][2 + i] + (H::THREE ? d1[n][i] : 0.f));
+        s[n][i] = (ok >> (n * 8 + c + i)) & 1 ? (H::THREE ? x : x * unscale) : -INFINITY;
+      }
+    float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    if (__any_sync(0xffffffffu, top > m + kLazy)) {
+      const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : exp2f(m - to);
+      m = to;
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < 2 * KD; j++) acc[j][0] *= f, acc[j][1] *= f;
+    }
+    float p[2][2];
+    uint32_t pa[4], pb[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+      p[n][0] = exp2_of(s[n][0], m);
+      p[n][1] = exp2_of(s[n][1], m);
+      l += p[n][0] + p[n][1];
+      pa[2 * n] = H::pack(p[n][0], p[n][1]);
+      const float2 f0 = H::unpack(pa[2 * n]);
+      const float u = p[n][0] - f0.x, v = p[n][1] - f0.y;
+      pa[2 * n + 1] = H::pack(u, v);
+      if constexpr (H::THREE) {
+        const float2 f1 = H::unpack(pa[2 * n + 1]);
+        pb[2 * n] = H::pack(u - f1.x, v - f1.y);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < KD; j++) {
+      uint32_t b[4];
+      ldmatrix4_trans(b, vs + j * 32);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        float d[4] = {};
+        H::mma(d, pa, b[2 * i], b[2 * i + 1]);
+        if constexpr (H::THREE) H::mma(d, pb, b[2 * i], b[2 * i + 1]);
+        acc[2 * j + i][0] += d[0] + d[2];
+        acc[2 * j + i][1] += d[1] + d[3];
+      }
+    }
+  }
+
+  __device__ void finish(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = (lane & 3) * 2, dim = a.kv.dim;
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    bool bad = !(fabsf(l) < INFINITY);
+#pragma unroll
+    for (int j = 0; j < 2 * KD; j++) bad |= !(fabsf(acc[j][0]) < INFINITY) || !(fabsf(acc[j][1]) < INFINITY);
+    if (__any_sync(0xffffffffu, bad && r < a.part)) {
+      attend_plain<T>(a, b, hc, j0, j1, rec);
+      return;
+    }
+    if (r < a.part) {
+      float* x = rec + r * (dim + 2);
+      if (c == 0) {
+        x[0] = m;
+        x[1] = l;
+      }
+#pragma unroll
+      for (int j = 0; j < 2 * KD; j++)
+        if (j * 8 < dim) {
+          x[2 + j * 8 + c] = acc[j][0];
+          x[3 + j * 8 + c] = acc[j][1];
+        }
+    }
+    __syncwarp();
+  }
+};
+
+// ------------------------------------------------------- fp32 caches (and wide 16-bit heads)
+//
+// LPR lanes share a row, each with CPL units of 16 bytes of it, so a warp treats 32 / LPR positions at
+// a time, R times per tile.  A lane copies exactly the units that it reads itself.  The R * GT partial
+// scores of a lane are summed over the lanes of a row by halving: each step exchanges half of the
+// values with a lane that keeps the other half, so 32 sums cost 31 shuffles and not 160, and each
+// lane ends with the scores that it turns into weights (no weight is computed twice).
+template <typename T, int LPR, int CPL, int GT>
+struct PathFma {
+  static constexpr int VE = 16 / (int)sizeof(T), KPW = 32 / LPR;
+  static constexpr int KT = LPR <= 16 ? 16 : CPL == 1 ? 8 : 4, R = KT / KPW;
+  static constexpr int WARPS = 8, UNIT = VE;
+  static constexpr bool RING = true;
+  static constexpr int TILE_BYTES = 2 * R * CPL * 512;
+  static constexpr int STAGE_BYTES = TILE_BYTES + KT * GT * 4;
+  static constexpr int STAGES = TILE_BYTES >= 8192 ? 2 : 4;
+  static constexpr int V = R * GT, NV = V > LPR ? V / LPR : 1;  // scores per lane
+  static constexpr int SAME = LPR / GT;                         // lanes of a row with scores of one head
+  static constexpr int COPIES = V < LPR ? LPR / V : 1;          // lanes of a row with the same score
+  static_assert(GT <= LPR && R % 4 == 0, "layout");
+
+  float q[GT][CPL * VE], acc[GT][CPL * VE], m, l;  // m, l: of this lane's head
+
+  __device__ static int lane_in() { return (threadIdx.x & 31) % LPR; }
+  __device__ static int group() { return (threadIdx.x & 31) / LPR; }
+  __device__ static int first() { return V >= LPR ? lane_in() * NV : lane_in() / COPIES; }  // score index g * R + r
+
+  __device__ void setup(const AttendArgs&, char*) {}
+
+  __device__ void begin(const AttendArgs& a, int b, int hc) {
+    const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * a.part, dim = a.kv.dim;
+#pragma unroll
+    for (int g = 0; g < GT; g++) {
+      const bool head = g < a.part && g0 + g < a.group;
+      const float* x = a.q + (size_t)b * a.qs + (size_t)(hk * a.group + (head ? g0 + g : 0)) * dim;
+#pragma unroll
+      for (int i = 0; i < CPL * VE; i++) {
+        const int d = (lane_in() + (i / VE) * LPR) * VE + i % VE;
+        q[g][i] = head && d < dim ? x[d] * a.scale : 0.f;
+        acc[g][i] = 0.f;
+      }
+    }
+    m = -INFINITY;
+    l = 0.f;
+  }
+
+  __device__ void issue(const AttendArgs& a, char* st, int lane, uint32_t row) {
+    const uint32_t dst = smem_u32(st) + lane * 16, units = a.kv.dim / VE;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const uint32_t at = __shfl_sync(0xffffffffu, row, r * KPW + group());
+#pragma unroll
+      for (int c = 0; c < CPL; c++) {
+        const uint32_t u = lane_in() + c * LPR;
+        const bool live = at != kNoRow && u < units;
+        const size_t off = live ? ((size_t)at + u) << 4 : 0;
+        cp_async16(dst + (r * CPL + c) * 512, (const char*)a.kc + off, live ? 16 : 0);
+        cp_async16(dst + ((R + r) * CPL + c) * 512, (const char*)a.vc + off, live ? 16 : 0);
+      }
+    }
+  }
+
+  static __device__ __forceinline__ void load(const char* at, float (&x)[CPL * VE]) {
+#pragma unroll
+    for (int c = 0; c < CPL; c++) {
+      const uint4 u = *reinterpret_cast<const uint4*>(at + c * 512);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if constexpr (VE == 4) {
+          x[c * VE + i] = __uint_as_float(w[i]);
+        } else {
+          const float2 f = Half2<T>::unpack(w[i]);
+          x[c * VE + 2 * i] = f.x;
+          x[c * VE + 2 * i + 1] = f.y;
+        }
+      }
+    }
+  }
+
+  template <int N, int O>
+  static __device__ __forceinline__ void halve(float* v) {
+    if constexpr (O > 0) {
+      if constexpr (N > 1) {
+        const bool up = (threadIdx.x & O) != 0;
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+          const float send = up ? v[i] : v[i + N / 2], keep = up ? v[i + N / 2] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, O);
+        }
+        halve<N / 2, O / 2>(v);
+      } else {
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], O);
+        halve<1, O / 2>(v);
+      }
+    }
+  }
+
+  __device__ void tile(const AttendArgs&, char* st, uint32_t ok) {
+    const int lane = threadIdx.x & 31;
+    float s[V];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      float k[CPL * VE];
+      load(st + r * CPL * 512 + lane * 16, k);
+#pragma unroll
+      for (int g = 0; g < GT; g++) {
+        float x = q[g][0] * k[0];
+#pragma unroll
+        for (int i = 1; i < CPL * VE; i++) x += q[g][i] * k[i];
+        s[g * R + r] = x;
+      }
+    }
+    halve<V, LPR / 2>(s);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int r = (first() + i) % R;
+      if (!((ok >> (r * KPW + group())) & 1)) s[i] = -INFINITY;
+      top = fmaxf(top, s[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < SAME; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+    for (int o = LPR; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (__any_sync(0xffffffffu, top > m + kLazy)) {
+      const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : exp2f(m - to);
+      m = to;
+      l *= f;
+#pragma unroll
+      for (int g = 0; g < GT; g++) {
+        const float fg = __shfl_sync(0xffffffffu, f, g * SAME);
+#pragma unroll
+        for (int i = 0; i < CPL * VE; i++) acc[g][i] *= fg;
+      }
+    }
+    float* ps = reinterpret_cast<float*>(st + TILE_BYTES) + group() * V;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const float p = exp2_of(s[i], m);
+      l += p;
+      ps[first() + i] = p;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int r4 = 0; r4 < R; r4 += 4) {
+      float p[GT][4];
+#pragma unroll
+      for (int g = 0; g < GT; g++) *reinterpret_cast<float4*>(p[g]) = *reinterpret_cast<const float4*>(ps + g * R + r4);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        float v[CPL * VE];
+        load(st + (R + r4 + r) * CPL * 512 + lane * 16, v);
+#pragma unroll
+        for (int g = 0; g < GT; g++)
+#pragma unroll
+          for (int i = 0; i < CPL * VE; i++) acc[g][i] += p[g][r] * v[i];
+      }
+    }
+  }
+
+  __device__ void finish(const AttendArgs& a, int, int, uint32_t, uint32_t, float* rec) {
+    const int dim = a.kv.dim;
+#pragma unroll
+    for (int o = 1; o < SAME; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+    for (int o = LPR; o < 32; o <<= 1) {
+      l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+      for (int g = 0; g < GT; g++)
+#pragma unroll
+        for (int i = 0; i < CPL * VE; i++) acc[g][i] += __shfl_xor_sync(0xffffffffu, acc[g][i], o);
+    }
+    if (group() == 0) {
+#pragma unroll
+      for (int g = 0; g < GT; g++) {
+        if (g >= a.part) continue;
+        float* x = rec + g * (dim + 2);
+        if (lane_in() == g * SAME) {
+          x[0] = m;
+          x[1] = l * (1.f / COPIES);
+        }
+#pragma unroll
+        for (int i = 0; i < CPL * VE; i++) {
+          const int d = (lane_in() + (i / VE) * LPR) * VE + i % VE;
+          if (d < dim) x[2 + d] = acc[g][i];
+        }
+      }
+    }
+    __syncwarp();
+  }
+};
+
+// ------------------------------------------------------------------------------ the kernel
+template <typename P>
+constexpr size_t ring_bytes() {
+  return (size_t)P::WARPS * P::STAGES * (P::STAGE_BYTES + 16);
+}
+
+template <typename P>
+__global__ void __launch_bounds__(P::WARPS * 32) k_paged_attend(const __grid_constant__ AttendArgs a) {
+  constexpr int KT = P::KT, WARPS = P::WARPS, THREADS = WARPS * 32;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ unsigned long long pre[kPrefix + 1];
+  __shared__ unsigned long long warp_tot[WARPS];
+  __shared__ long long seg_id[WARPS][2];  // first tile (on the line) of the sequence part in each record, -1: none
+  __shared__ int seg_b[WARPS][2], seg_hc[WARPS][2];
+  __shared__ unsigned s_old[2];
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, dim = a.kv.dim;
+  const int hcs = a.kv.kv_heads * a.chunks;
+  const int rf = rec_floats(a);
+  float* recs = reinterpret_cast<float*>(smem + ring_bytes<P>());
+  char* ring = smem + (size_t)w * P::STAGES * (P::STAGE_BYTES + 16);
+
+  // Tiles before every `step`-th sequence, for the whole batch.
+  const int step = (a.kv.batch + kPrefix - 1) / kPrefix, n_pre = (a.kv.batch + step - 1) / step;
+  {
+    constexpr int PER = (kPrefix + THREADS - 1) / THREADS;
+    unsigned long long mine[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int e = tid * PER + i;
+      mine[i] = sum;
+      if (e < n_pre)
+        for (int b = e * step; b < min(a.kv.batch, (e + 1) * step); b++) {
+          if (a.kv.lens[b] > a.kv.max_pages * a.kv.page_size && blockIdx.x == 0)
+            atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
+          const Seq s = seq_of<KT>(a, b);
+          sum += (unsigned long long)(s.t1 - s.t0) * hcs;
+        }
+    }
+    unsigned long long inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) warp_tot[w] = inc;
+    __syncthreads();
+    unsigned long long base = inc - sum;
+    for (int i = 0; i < w; i++) base += warp_tot[i];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int e = tid * PER + i;
+      if (e < n_pre) pre[e] = base + mine[i];
+    }
+    if (tid == THREADS - 1) pre[n_pre] = base + sum;
+  }
+  if (tid < WARPS * 2) seg_id[tid >> 1][tid & 1] = -1;
+  __syncthreads();
+  const unsigned long long total = pre[n_pre];
+
+  // Idle sequences: zeros.
+  for (int b = blockIdx.x; b < a.kv.batch; b += gridDim.x) {
+    if (seq_of<KT>(a, b).n) continue;
+    for (int e = tid; e < a.heads * dim; e += THREADS) a.out[(size_t)b * a.os + e] = 0.f;
+    if (a.lse)
+      for (int e = tid; e < a.heads; e += THREADS) a.lse[(size_t)b * a.heads + e] = -INFINITY;
+  }
+
+  // This block's stretch of the line, and this warp's.
+  const unsigned long long least = (unsigned long long)WARPS * a.min_tiles;
+  const unsigned long long want = (total + least - 1) / least;
+  const unsigned blocks = want < gridDim.x ? (unsigned)want : gridDim.x;
+  if (blockIdx.x >= blocks) return;
+  const unsigned long long lo = total * blockIdx.x / blocks, hi = total * (blockIdx.x + 1) / blocks;
+  const unsigned long long wlo = lo + (hi - lo) * w / WARPS, whi = lo + (hi - lo) * (w + 1) / WARPS;
+
+  if (wlo < whi) {
+    P path;
+    path.setup(a, ring);
+    Walk<KT> at;  // where the softmax is
+    {
+      int l = 0, r = n_pre - 1;
+      while (l < r) {
+        const int mid = (l + r + 1) >> 1;
+        if (pre[mid] <= wlo)
+          l = mid;
+        else
+          r = mid - 1;
+      }
+      unsigned long long u = pre[l];
+      int b = l * step;
+      Seq s = seq_of<KT>(a, b);
+      while (u + (unsigned long long)(s.t1 - s.t0) * hcs <= wlo) {
+        u += (unsigned long long)(s.t1 - s.t0) * hcs;
+        s = seq_of<KT>(a, ++b);
+      }
+      const unsigned long long in = wlo - u;
+      at.s = s;
+      at.b = b;
+      at.hc = (int)(in / (s.t1 - s.t0));
+      at.t = s.t0 + (uint32_t)(in % (s.t1 - s.t0));
+    }
+    Walk<KT> ahead = at;  // where the copies are
+    const unsigned long long count = whi - wlo;
+    unsigned long long issued = 0;
+    // Page of this lane's row of the next tile to issue, fetched a tile early.
+    uint32_t id = kNoRow, slot = 0;
+    bool live = false;
+    auto look = [&]() {
+      const uint32_t j = ahead.t * KT + lane;
+      live = lane < KT && j >= ahead.s.first && j < ahead.s.n;
+      const uint32_t pg = live ? page_of(a, j) : 0;
+      slot = j - pg * a.kv.page_size;
+      id = live ? a.kv.table[(size_t)ahead.b * a.kv.max_pages + pg] : kNoRow;
+    };
+    look();
+    auto issue = [&]() {
+      if (issued < count) {
+        uint32_t row = kNoRow;
+        if (live) {
+          if (id < a.kv.n_pages) {
+            if constexpr (P::RING)
+              row = (uint32_t)(((size_t)id * a.kv.page_stride + (size_t)(ahead.hc / a.chunks) * a.kv.head_stride +
+                                (size_t)slot * a.kv.slot_stride) /
+                               P::UNIT);
+            else
+              row = 0;
+          } else {
+            atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
+          }
+        }
+        const uint32_t ok = __ballot_sync(0xffffffffu, row != kNoRow);
+        char* st = ring + (issued % P::STAGES) * (P::STAGE_BYTES + 16);
+        if constexpr (P::RING) {
+          if (lane == 0) *reinterpret_cast<uint32_t*>(st + P::STAGE_BYTES) = ok;
+        }
+        path.issue(a, st, lane, row);
+        issued++;
+        if (issued < count) {
+          ahead.next(a, hcs);
+          look();
+        }
+      }
+      if constexpr (P::RING) cp_commit();
+    };
+    for (int i = 0; i < P::STAGES - 1; i++) issue();
+    uint32_t part_t = at.t;  // where this warp's share of the current sequence part begins
+    path.begin(a, at.b, at.hc);
+    for (unsigned long long i = 0; i < count; i++) {
+      issue();
+      if constexpr (P::RING) {
+        cp_wait<P::STAGES - 1>();
+        __syncwarp();
+        char* st = ring + (i % P::STAGES) * (P::STAGE_BYTES + 16);
+        path.tile(a, st, *reinterpret_cast<uint32_t*>(st + P::STAGE_BYTES));
+        __syncwarp();
+      }
+      const bool ends = at.t + 1 == at.s.t1;
+      if (ends || i + 1 == count) {
+        const bool starts = part_t == at.s.t0;
+        const int which = starts ? 1 : 0;
+        float* rec = recs + (w * 2 + which) * rf;
+        path.finish(a, at.b, at.hc, max(at.s.first, part_t * KT), min(at.s.n, (at.t + 1) * KT), rec);
+        if (starts && ends) {
+          const int hk = at.hc / a.chunks, g0 = (at.hc - hk * a.chunks) * a.part;
+          const int n_g = min(a.part, a.group - g0), h0 = hk * a.group + g0;
+          for (int e = lane; e < n_g * dim; e += 32) {
+            const int g = e / dim, d = e - g * dim;
+            store_out(a, at.b, h0 + g, d, rec[g * (dim + 2) + 2 + d], rec[g * (dim + 2) + 1]);
+          }
+          if (lane < n_g) store_lse(a, at.b, h0 + lane, rec[lane * (dim + 2)], rec[lane * (dim + 2) + 1]);
+          __syncwarp();
+        } else if (lane == 0) {
+          seg_id[w][which] = (long long)(wlo + i) - (long long)(at.t - at.s.t0);
+          seg_b[w][which] = at.b;
+          seg_hc[w][which] = at.hc;
+        }
+        if (i + 1 < count) {
+          at.next(a, hcs);
+          part_t = at.t;
+          path.begin(a, at.b, at.hc);
+        }
+      } else {
+        at.t++;
+      }
+    }
+  }
+  __syncthreads();
+
+  // Join the warps' records, in the order of positions; records r = 2 w + which of one sequence part
+  // follow one another.  A part that lies in this block whole is done; the block's first may have
+  // begun before it (slot 0), its last may go on behind it (slot 1).
+  int open_first[2] = {-1, -1}, open_b[2], open_hc[2], open_parts[2];
+  for (int r = 0; r < 2 * WARPS; r++) {
+    const long long id = seg_id[r >> 1][r & 1];
+    if (id < 0) continue;
+    int end = r + 1;
+    for (int e = r + 1; e < 2 * WARPS; e++) {
+      const long long x = seg_id[e >> 1][e & 1];
+      if (x >= 0 && x != id) break;
+      if (x == id) end = e + 1;
+    }
+    const int b = seg_b[r >> 1][r & 1], hc = seg_hc[r >> 1][r & 1];
+    const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * a.part;
+    const int n_g = min(a.part, a.group - g0), h0 = hk * a.group + g0;
+    const Seq s = seq_of<KT>(a, b);
+    const unsigned long long u0 = id, u1 = u0 + (s.t1 - s.t0);
+    const bool before = u0 < lo, behind = u1 > hi;
+    const int slot = before ? 0 : 1;
+    float* part = a.partial + (size_t)(blockIdx.x * 2 + slot) * rf;
+    for (int e = tid; e < n_g * dim; e += THREADS) {
+      const int g = e / dim, d = e - g * dim;
+      float top = -INFINITY;
+      for (int x = r; x < end; x++)
+        if (seg_id[x >> 1][x & 1] == id) top = fmaxf(top, recs[x * rf + g * (dim + 2)]);
+      float o = 0.f, l = 0.f;
+      for (int x = r; x < end; x++) {
+        if (seg_id[x >> 1][x & 1] != id) continue;
+        const float* rec = recs + x * rf + g * (dim + 2);
+        const float f = weight_of(rec[0], rec[1], top);
+        l += f * rec[1];
+        o += f * rec[2 + d];
+      }
+      if (before || behind) {
+        __stcg(part + g * (dim + 2) + 2 + d, o);
+        if (d == 0) {
+          __stcg(part + g * (dim + 2), top);
+          __stcg(part + g * (dim + 2) + 1, l);
+        }
+      } else {
+        store_out(a, b, h0 + g, d, o, l);
+        if (d == 0) store_lse(a, b, h0 + g, top, l);
+      }
+    }
+    if (before || behind) {
+      // blocks that hold tiles u0 and u1 - 1
+      const int c0 = (int)(((u0 + 1) * blocks - 1) / total), c1 = (int)((u1 * blocks - 1) / total);
+      open_first[slot] = c0;
+      open_parts[slot] = c1 - c0 + 1;
+      open_b[slot] = b;
+      open_hc[slot] = hc;
+    }
+    r = end - 1;
+  }
+  if (open_first[0] < 0 && open_first[1] < 0) return;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+      if (open_first[i] >= 0) s_old[i] = atomicAdd(&a.counters[open_first[i]], 1u);
+  }
+  __syncthreads();
+  float* wt = reinterpret_cast<float*>(smem);  // [parts][heads of the part] weights, then the sums
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    if (open_first[i] < 0 || s_old[i] + 1 != (unsigned)open_parts[i]) continue;
+    // the last of its blocks to arrive: every partial result is there
+    __threadfence();
+    if (tid == 0) a.counters[open_first[i]] = 0;
+    const int c0 = open_first[i], parts = open_parts[i], b = open_b[i], hc = open_hc[i];
+    const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * a.part;
+    const int n_g = min(a.part, a.group - g0), h0 = hk * a.group + g0;
+    const float* p0 = a.partial + ((size_t)c0 * 2 + 1) * rf;  // block c0's slot 1, then slot 0 of the next ones
+    auto at = [&](int x) { return x == 0 ? p0 : a.partial + (size_t)(c0 + x) * 2 * rf; };
+    __syncthreads();
+    for (int g = w; g < n_g; g += WARPS) {
+      float top = -INFINITY, sum = 0.f;
+      for (int x = lane; x < parts; x += 32) top = fmaxf(top, __ldcg(at(x) + g * (dim + 2)));
+      top = warp_max(top);
+      for (int x = lane; x < parts; x += 32) {
+        const float* p = at(x) + g * (dim + 2);
+        const float l = __ldcg(p + 1), f = weight_of(__ldcg(p), l, top);
+        wt[x * n_g + g] = f;
+        sum += f * l;
+      }
+      sum = warp_sum(sum);
+      if (lane == 0) {
+        wt[parts * n_g + g] = sum;
+        store_lse(a, b, h0 + g, top, sum);
+      }
+    }
+    __syncthreads();
+    for (int e = tid; e < n_g * dim; e += THREADS) {
+      const int g = e / dim, d = e - g * dim;
+      float o = 0.f;
+#pragma unroll 8
+      for (int x = 0; x < parts; x++) o += wt[x * n_g + g] * __ldcg(at(x) + g * (dim + 2) + 2 + d);
+      store_out(a, b, h0 + g, d, o, wt[parts * n_g + g]);
+    }
+    __syncthreads();
+  }
+}
+
+int sm_count(int device, int* out) {
+  static std::atomic<int> known[64];
+  int n = known[device & 63].load(std::memory_order_relaxed);
+  if (!n) {
+    TURT_CHECK_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
+    known[device & 63].store(n, std::memory_order_relaxed);
+  }
+  *out = n;
+  return OK;
+}
+
+template <typename P>
+int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
+  static std::atomic<uint64_t> done{0};
+  a.part = part;
+  a.chunks = (a.group + part - 1) / part;
+  a.min_tiles = 2;
+  int sms = 0;
+  RC(sm_count(ctx->device, &sms));
+  const size_t rec = (size_t)P::WARPS * 2 * part * (a.kv.dim + 2) * 4;
+  // the join of blocks keeps a weight per partial result and head
+  const size_t smem = std::max(ring_bytes<P>() + rec, (size_t)(kMaxBlocks + 1) * part * 4);
+  RC(smem_attr_per_device(done, k_paged_attend<P>, 218 * 1024));
+  TURT_REQUIRE(smem <= 218 * 1024, "paged_attention: shared memory");
+  static std::atomic<int> regs{0};
+  if (!regs.load(std::memory_order_relaxed)) {
+    cudaFuncAttributes at;
+    TURT_CHECK_CUDA(cudaFuncGetAttributes(&at, k_paged_attend<P>));
+    regs.store(at.numRegs, std::memory_order_relaxed);
+  }
+  const int per_sm = smem <= 103 * 1024 && regs.load(std::memory_order_relaxed) <= 128 ? 2 : 1;
+  const int grid = std::min(kMaxBlocks, sms * per_sm);
+  k_paged_attend<P><<<grid, P::WARPS * 32, smem, ctx->stream>>>(a);
+  TURT_LAUNCH_CHECK();
+  return OK;
+}
+
+// Whether rows are whole 16-byte units on 16-byte boundaries whose numbers fit 32 bits.
+template <typename T>
+bool in_units(const AttendArgs& a) {
+  const size_t n = 16 / sizeof(T);
+  const PagedLayout& kv = a.kv;
+  const size_t last = (kv.n_pages - 1) * kv.page_stride + (kv.kv_heads - 1) * kv.head_stride +
+                      (kv.page_size - 1) * kv.slot_stride;
+  return aligned16(a.kc) && aligned16(a.vc) && kv.dim % n == 0 && kv.page_stride % n == 0 && kv.head_stride % n == 0 &&
+         kv.slot_stride % n == 0 && last / n < kNoRow;
+}
+
+template <typename T, int LPR, int CPL, int MOST>
+int attend_fma(turt_ctx* ctx, const AttendArgs& a) {
+  if (a.group == 1) return attend_launch<PathFma<T, LPR, CPL, 1>>(ctx, a, 1);
+  if (a.group == 2) return attend_launch<PathFma<T, LPR, CPL, 2>>(ctx, a, 2);
+  if (a.group <= 4 || MOST == 4) return attend_launch<PathFma<T, LPR, CPL, 4>>(ctx, a, std::min(a.group, 4));
+  if constexpr (MOST == 8) return attend_launch<PathFma<T, LPR, CPL, 8>>(ctx, a, std::min(a.group, 8));
+  return ERR_UNSUPPORTED;
+}
+
+template <typename T>
+int attend_typed(turt_ctx* ctx, const AttendArgs& a) {
+  const int dim = a.kv.dim;
+  if (!in_units<T>(a)) return attend_launch<PathPlain<T>>(ctx, a, 1);
+  if constexpr (sizeof(T) == 4) {
+    if (dim <= 32) return attend_fma<T, 8, 1, 8>(ctx, a);
+    if (dim <= 64) return attend_fma<T, 16, 1, 8>(ctx, a);
+    if (dim <= 128) return attend_fma<T, 32, 1, 8>(ctx, a);
+    return attend_fma<T, 32, 2, 4>(ctx, a);
+  } else {
+    const int part = std::min(a.group, kGroup);
+    if (dim <= 32) return attend_launch<PathMma<T, 2>>(ctx, a, part);
+    if (dim <= 64) return attend_launch<PathMma<T, 4>>(ctx, a, part);
+    if (dim <= 80) return attend_launch<PathMma<T, 5>>(ctx, a, part);
+    if (dim <= 96) return attend_launch<PathMma<T, 6>>(ctx, a, part);
+    if (dim <= 128) return attend_launch<PathMma<T, 8>>(ctx, a, part);
+    return attend_fma<T, 32, 1, 4>(ctx, a);
+  }
+}
+
+constexpr size_t kCounterBytes = kMaxBlocks * 4;
+
+}  // namespace
+}  // namespace turt
+
+using namespace turt;
+
+extern "C" int turt_paged_attention_workspace(const turt_paged_kv* kv, int n_head, size_t* bytes) {
+  PagedLayout p;
+  RC(paged_layout(kv, &p));
+  TURT_REQUIRE(bytes, "paged_attention_workspace: null bytes");
+  TURT_REQUIRE(n_head > 0 && n_head % kv->n_kv_head == 0, "paged_attention: n_head must be a multiple of n_kv_head");
+  const int part = std::min(kGroup, n_head / kv->n_kv_head);
+  *bytes = kCounterBytes + (size_t)kMaxBlocks * 2 * part * (kv->head_dim + 2) * 4;
+  return OK;
+}
+
+extern "C" int turt_paged_attention(turt_ctx* ctx, const turt_paged_kv* kv, const float* q, size_t q_stride, float* out,
+                                    size_t out_stride, float* lse, int n_head, float scale, int window, void* workspace,
+                                    size_t workspace_bytes) {
+  AttendArgs a;
+  size_t need = 0;
+  RC(paged_layout(kv, &a.kv));
+  RC(turt_paged_attention_workspace(kv, n_head, &need));
+  const size_t wide = (size_t)n_head * kv->head_dim;
+  TURT_REQUIRE(kv->batch == 0 || (q && out), "paged_attention: null pointer");
+  TURT_REQUIRE(kv->batch <= 1 || (q_stride >= wide && out_stride >= wide),
+               "paged_attention: row strides below the row width");
+  TURT_REQUIRE(window >= 0, "paged_attention: negative window");
+  TURT_REQUIRE(isfinite(scale), "paged_attention: scale must be finite");
+  TURT_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)lse) % 4 == 0, "paged_attention: misaligned pointer");
+  TURT_REQUIRE(workspace && workspace_bytes >= need && aligned16(workspace),
+               "paged_attention: workspace missing, misaligned or smaller than turt_paged_attention_workspace says");
+  TURT_REQUIRE(ctx, "null context");
+  TURT_CHECK_CUDA(cudaSetDevice(ctx->device));
+  if (kv->batch == 0) return OK;
+  a.kc = kv->k, a.vc = kv->v;
+  a.q = q, a.out = out, a.lse = lse;
+  a.qs = q_stride, a.os = out_stride;
+  a.heads = n_head, a.group = n_head / kv->n_kv_head, a.window = window;
+  a.scale = (float)(scale * 1.4426950408889634);
+  // division by the page size: mul = ceil(2^(31 + s) / d) with 2^s >= d is exact for positions < 2^31
+  int s = 0;
+  while ((1ll << s) < kv->page_size) s++;
+  a.div_mul = (uint32_t)(((1ull << (31 + s)) + kv->page_size - 1) / kv->page_size);
+  a.div_shift = 31 + s;
+  a.counters = static_cast<uint32_t*>(workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+  a.flags = ctx->flags;
+  if (kv->dtype == TURT_CACHE_F32) return attend_typed<float>(ctx, a);
+  if (kv->dtype == TURT_CACHE_F16) return attend_typed<__half>(ctx, a);
+  return attend_typed<__nv_bfloat16>(ctx, a);
+}
