@@ -1154,9 +1154,7 @@ __global__ void k_gemm_simt(const float* __restrict__ A, const float* __restrict
 }
 
 // ------------------------------------------------------------ host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+typedef TensorMapEncode EncodeTiledFn;
 
 EncodeTiledFn get_encode() {
   static EncodeTiledFn fn = nullptr;
@@ -1467,6 +1465,8 @@ void gemm_set_tile_override(int bn, int pair) {
   g_tile_override.store(bn);
   g_pair_override.store(pair);
 }
+
+TensorMapEncode tensor_map_encode() { return get_encode(); }
 
 int tensor_map_f32(CUtensorMap* map, const GemmOperand& op, long inner, long rows, int bdiv, int batch,
                    int box_inner, int box_rows, bool mn_major) {

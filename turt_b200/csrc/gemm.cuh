@@ -84,6 +84,12 @@ int gemm_tf32(cudaStream_t stream, int M, int N, int K, int batch, const GemmOpe
               const GemmOperand& B, const GemmEpi& epi, int* dev_flags, int precision = GEMM_TF32X3,
               int force_splits = 0);
 
+// The driver's cuTensorMapEncodeTiled, or null where it cannot be found.
+typedef CUresult (*TensorMapEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+TensorMapEncode tensor_map_encode();
+
 // 4-D TMA tensor map over operand `op` viewed as [batch / bdiv][bdiv][rows][inner] (the same
 // view gemm_tf32 uses), with a box of box_inner x box_rows floats: K-major boxes 32 floats wide
 // take the 128-byte swizzle, MN-major ones the 128-byte swizzle with 32-byte atoms.

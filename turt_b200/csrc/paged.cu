@@ -44,6 +44,10 @@ int paged_layout(const turt_paged_kv* kv, PagedLayout* out) {
                      (kv->n_pages == 1 || p.page_stride >= d),
                  "paged cache: strides let positions overlap");
   }
+  // strides of single entries are never used: legal values
+  if (kv->page_size == 1) p.slot_stride = d;
+  if (kv->n_kv_head == 1) p.head_stride = p.slot_stride;
+  if (kv->n_pages == 1) p.page_stride = p.slot_stride;
   p.table = kv->page_table;
   p.lens = kv->lens;
   p.n_pages = kv->n_pages;

@@ -6,9 +6,9 @@
 // the memory bandwidth.  The positions of all sequences and key heads form one line of tiles, cut
 // into equal stretches, one per warp of a grid that fills the GPU once: ragged lengths, one long
 // sequence and many short ones load all warps alike, whatever the lengths are (they are read on the
-// device).  A warp streams its tiles through a ring of shared memory of its own with 16-byte
-// asynchronous copies, so nothing but its own copies holds it up; it runs the online softmax of its
-// stretch in registers.  A part of a sequence that a warp did not see whole is joined with its
+// device).  A warp streams its tiles through a ring of shared memory of its own, filled by bulk tensor
+// copies that one lane issues, so nothing but its own copies holds it up; it runs the online softmax
+// of its stretch in registers.  A part of a sequence that a warp did not see whole is joined with its
 // neighbours': first inside the block, then by the last block to arrive, always in the order of
 // positions.
 #include <math.h>
@@ -16,7 +16,9 @@
 #include <algorithm>
 
 #include "ctx.cuh"
+#include "gemm.cuh"
 #include "paged.cuh"
+#include "tcgen05.cuh"
 
 namespace turt {
 namespace {
@@ -25,7 +27,7 @@ constexpr int kMaxBlocks = 512;           // counters and partial results in the
 constexpr int kPrefix = 1024;             // entries of the tile prefix held in shared memory
 constexpr int kGroup = 8;                 // heads of a group that a warp treats at once, at most
 constexpr float kLazy = 8.0f;             // the running max moves when it is this far behind (log2)
-constexpr uint32_t kNoRow = 0xFFFFFFFFu;  // no cached position behind this row of a tile
+constexpr int kWaitSite = 40;             // reported when a copy's wait runs out
 
 struct AttendArgs {
   PagedLayout kv;
@@ -40,9 +42,12 @@ struct AttendArgs {
   uint32_t div_mul;  // position / page_size = position * div_mul >> div_shift (positions < 2^31)
   int div_shift;
   int min_tiles;     // tiles per warp, at least
+  int box_rows;      // positions per copy
+  int page_tiles;    // tiles per page where tiles do not cross pages, 0: any KT positions are a tile
   uint32_t* counters;
   float* partial;
   int* flags;
+  int dtype;
 };
 
 __device__ __forceinline__ uint32_t page_of(const AttendArgs& a, uint32_t j) {
@@ -51,27 +56,46 @@ __device__ __forceinline__ uint32_t page_of(const AttendArgs& a, uint32_t j) {
 
 __device__ __forceinline__ float exp2_of(float s, float m) { return exp2f(s - (m == -INFINITY ? 0.f : m)); }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ unsigned long long div64(unsigned long long x, unsigned long long y) {
+  return (x | y) >> 32 ? x / y : (unsigned)x / (unsigned)y;
 }
 
-// The positions that sequence b attends to: [first, n) in tiles [t0, t1) of KT.
+// The positions that sequence b attends to: [first, n) in tiles [t0, t1).  A tile is KT positions, or,
+// where KT (in pieces of box_rows) does not divide the page size, KT slots of one page.
 struct Seq {
   uint32_t n, first, t0, t1;
 };
+template <int KT>
+__device__ __forceinline__ uint32_t tile_of(const AttendArgs& a, uint32_t j) {
+  if (!a.page_tiles) return j / KT;
+  const uint32_t pg = page_of(a, j);
+  return pg * a.page_tiles + (j - pg * a.kv.page_size) / KT;
+}
+// Positions [j0, j1) of tile t.
+template <int KT>
+__device__ __forceinline__ void tile_span(const AttendArgs& a, uint32_t t, uint32_t* j0, uint32_t* j1) {
+  if (!a.page_tiles) {
+    *j0 = t * KT;
+    *j1 = *j0 + KT;
+  } else {
+    const uint32_t pg = t / a.page_tiles;
+    *j0 = pg * a.kv.page_size + (t - pg * a.page_tiles) * KT;
+    *j1 = min(*j0 + KT, (pg + 1) * a.kv.page_size);
+  }
+}
 template <int KT>
 __device__ __forceinline__ Seq seq_of(const AttendArgs& a, int b) {
   Seq s;
   s.n = a.kv.lens[b];
   if (s.n > a.kv.max_pages * a.kv.page_size) s.n = 0;  // flagged where the batch is scanned
   s.first = a.window > 0 && s.n > (uint32_t)a.window ? s.n - a.window : 0;
-  s.t0 = s.first / KT;
-  s.t1 = (s.n + KT - 1) / KT;
+  s.t0 = s.t1 = 0;
+  if (s.n) {
+    s.t0 = tile_of<KT>(a, s.first);
+    s.t1 = tile_of<KT>(a, s.n - 1) + 1;
+  }
   return s;
 }
 
@@ -157,16 +181,16 @@ __device__ __noinline__ void attend_plain(const AttendArgs& a, int b, int hc, ui
 }
 
 // Paths: how a warp treats the tiles of its stretch.
-//   issue(stage, row, ok)   starts the copies of a tile; lane r < KT holds row r's place in 16-byte units
 //   begin / tile / finish   the softmax of one part of a sequence; finish leaves its record in rec
+//   A tile lies in its stage of the ring as KT rows of keys and then KT of values, in slabs of SLAB
+//   elements (a slab holds all KT rows); `ok` has a bit for each row that is attended to, and the
+//   value rows without one are zero.
 // ------------------------------------------------------------------------------- any layout
 template <typename T>
 struct PathPlain {
   static constexpr int KT = 16, WARPS = 8, STAGES = 1, STAGE_BYTES = 0;
   static constexpr bool RING = false;
-  __device__ void setup(const AttendArgs&, char*) {}
   __device__ void begin(const AttendArgs&, int, int) {}
-  __device__ void issue(const AttendArgs&, char*, int, uint32_t) {}
   __device__ void tile(const AttendArgs&, char*, uint32_t) {}
   __device__ void finish(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
     attend_plain<T>(a, b, hc, j0, j1, rec);
@@ -179,8 +203,9 @@ struct PathPlain {
 // (8 at most) as rows.  Only the cache is 16-bit: q and the weights p are fp32 and go in as a sum of
 // 16-bit parts, one part in rows 0-7 and the next in rows 8-15 of the same product, so the unused
 // half of the rows buys the precision: fp16 takes two parts (22 bits; q scaled per head to [1, 2)
-// by a power of two), bf16 three (24 bits; the third in a product of its own).  The thread that
-// holds row r also holds row r + 8, so the parts of a score and of an output meet in one register,
+// by a power of two), bf16 three (24 bits): up to four heads have the second in rows 4-7 and the third
+// in rows 8-11, more heads the third in a product of its own.  The thread that holds row r also holds
+// row r + 8 (and the one 16 lanes on row r + 4), so the parts of a score meet after a shuffle at most,
 // and the scores are where the next product wants p.  Each tile's product is added to the running
 // output in fp32 outside the tensor cores, whose own accumulation truncates.
 // Infinities and NaN break the parts (0 * inf): a stretch that ends in a non-finite result is done
@@ -195,11 +220,11 @@ struct Half2<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                             const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
 };
 template <>
@@ -212,54 +237,65 @@ struct Half2<__nv_bfloat16> {
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
   }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                             const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 
-// KD: steps of 16 elements that cover head_dim (a multiple of 8).
-template <typename T, int KD>
+// KD: steps of 16 elements that cover head_dim (a multiple of 8).  QUAD: at most four heads.
+template <typename T, int KD, bool QUAD>
 struct PathMma {
   using H = Half2<T>;
-  static constexpr int KT = 16, WARPS = 8, UNIT = 8;
-  static constexpr bool RING = true;
-  // rows an odd number of 16-byte units apart: the eight rows of an ldmatrix fall into different banks
-  static constexpr int PITCH = (2 * KD + 1) * 16;
-  static constexpr int STAGE_BYTES = 2 * KT * PITCH;
-  static constexpr int STAGES = KD >= 6 ? 2 : KD >= 4 ? 3 : 4;
+  static constexpr int KT = 16, WARPS = 8;
+  static constexpr bool RING = true, SWIZZLE = true;
+  static constexpr bool SPLIT = QUAD && H::THREE;    // parts in rows r, r + 4, r + 8
+  static constexpr bool EXTRA = !QUAD && H::THREE;   // a product for the third part
+  // slabs of 16 rows of 128 bytes whose 16-byte units are exchanged (unit ^ row % 8): the eight rows of
+  // an ldmatrix fall into different banks
+  static constexpr int SLAB = 64, SLABS = (KD + 3) / 4, SLAB_BYTES = KT * SLAB * 2;
+  static constexpr int STAGE_BYTES = 2 * SLABS * SLAB_BYTES;
+  static constexpr int STAGES = SLABS == 2 ? 2 : 4;
 
-  uint32_t qa[KD][4], qb[H::THREE ? KD : 1][2];
+  uint32_t qa[KD][4], qb[EXTRA ? KD : 1][2];
   float acc[2 * KD][2], m, l, unscale;
-  uint32_t units, div;  // 16-byte units of a row; e / units = e * div >> 16 for e < 256
 
-  __device__ void setup(const AttendArgs& a, char* ring) {
-    units = a.kv.dim / 8;
-    div = (65536 + units - 1) / units;
-    if (units < 2 * KD)  // the copies leave the padding of a row as it is: zero
-      for (int s = 0; s < STAGES; s++)
-        for (int e = (threadIdx.x & 31) * 16; e < STAGE_BYTES; e += 512)
-          *reinterpret_cast<uint4*>(ring + s * (STAGE_BYTES + 16) + e) = make_uint4(0, 0, 0, 0);
-    __syncwarp();
+  // The parts of (u, v) for rows r and r + 8 of a product, and the third part's own.
+  static __device__ __forceinline__ void parts(float u, float v, uint32_t& x, uint32_t& y, uint32_t& z) {
+    const uint32_t p0 = H::pack(u, v);
+    const float2 f0 = H::unpack(p0);
+    u -= f0.x, v -= f0.y;
+    const uint32_t p1 = H::pack(u, v);
+    x = p0, y = p1;
+    if constexpr (H::THREE) {
+      const float2 f1 = H::unpack(p1);
+      const uint32_t p2 = H::pack(u - f1.x, v - f1.y);
+      if constexpr (SPLIT) {
+        const bool second = (threadIdx.x & 16) != 0;
+        x = second ? p1 : p0;
+        y = second ? 0u : p2;
+      }
+      z = p2;
+    }
   }
 
+  __device__ static int row() { return SPLIT ? (threadIdx.x & 15) >> 2 : (threadIdx.x & 31) >> 2; }
+
   __device__ void begin(const AttendArgs& a, int b, int hc) {
-    const int lane = threadIdx.x & 31, r = lane >> 2, c = (lane & 3) * 2, dim = a.kv.dim;
+    const int r = row(), c = (threadIdx.x & 3) * 2, dim = a.kv.dim;
     const int hk = hc / a.chunks, g = (hc - hk * a.chunks) * a.part + r;
     const bool head = r < a.part && g < a.group;
     const float* q = a.q + (size_t)b * a.qs + (size_t)(hk * a.group + (head ? g : 0)) * dim;
@@ -289,17 +325,9 @@ struct PathMma {
     for (int k = 0; k < KD; k++)
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        float u = x[k][2 * i] * up, v = x[k][2 * i + 1] * up;
-        const uint32_t p0 = H::pack(u, v);
-        const float2 f0 = H::unpack(p0);
-        u -= f0.x, v -= f0.y;
-        const uint32_t p1 = H::pack(u, v);
-        qa[k][2 * i] = p0;
-        qa[k][2 * i + 1] = p1;
-        if constexpr (H::THREE) {
-          const float2 f1 = H::unpack(p1);
-          qb[k][i] = H::pack(u - f1.x, v - f1.y);
-        }
+        uint32_t z = 0;
+        parts(x[k][2 * i] * up, x[k][2 * i + 1] * up, qa[k][2 * i], qa[k][2 * i + 1], z);
+        if constexpr (EXTRA) qb[k][i] = z;
       }
 #pragma unroll
     for (int j = 0; j < 2 * KD; j++) acc[j][0] = acc[j][1] = 0.f;
@@ -307,36 +335,22 @@ struct PathMma {
     l = 0.f;
   }
 
-  __device__ void issue(const AttendArgs& a, char* st, int lane, uint32_t row) {
-    const uint32_t dst = smem_u32(st);
-#pragma unroll
-    for (int i = 0; i < KD; i++) {
-      const uint32_t e = i * 32 + lane, rr = (e * div) >> 16, u = e - rr * units;
-      const uint32_t at = __shfl_sync(0xffffffffu, row, rr & 15);
-      if (rr < KT) {
-        const size_t off = at == kNoRow ? 0 : ((size_t)at << 4) + u * 16;
-        const uint32_t n = at == kNoRow ? 0 : 16;
-        cp_async16(dst + rr * PITCH + u * 16, (const char*)a.kc + off, n);
-        cp_async16(dst + (KT + rr) * PITCH + u * 16, (const char*)a.vc + off, n);
-      }
-    }
-  }
-
   __device__ void tile(const AttendArgs&, char* st, uint32_t ok) {
     const int lane = threadIdx.x & 31, c = (lane & 3) * 2;
-    const uint32_t ks = smem_u32(st) + ((lane & 7) + (lane >> 4) * 8) * PITCH + ((lane >> 3) & 1) * 16;
-    const uint32_t vs = smem_u32(st) + (KT + (lane & 15)) * PITCH + (lane >> 4) * 16;
+    const uint32_t ks = smem_u32(st) + ((lane & 7) + (lane >> 4) * 8) * 128, ku = (lane >> 3) & 1;
+    const uint32_t vs = smem_u32(st) + SLABS * SLAB_BYTES + (lane & 15) * 128, vu = lane >> 4, sw = lane & 7;
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
     float d0[2][4] = {}, d1[2][4] = {};
 #pragma unroll
     for (int k = 0; k < KD; k++) {
       uint32_t b[4];
-      ldmatrix4(b, ks + k * 32);
-      H::mma(d0[0], qa[k], b[0], b[1]);
-      H::mma(d0[1], qa[k], b[2], b[3]);
-      if constexpr (H::THREE) {
+      ldmatrix4(b, ks + k / 4 * SLAB_BYTES + (((k % 4 * 2 + ku) ^ sw) << 4));
+      H::mma(d0[0], qa[k], b[0], b[1], d0[0]);
+      H::mma(d0[1], qa[k], b[2], b[3], d0[1]);
+      if constexpr (EXTRA) {
         const uint32_t low[4] = {qb[k][0], 0, qb[k][1], 0};
-        H::mma(d1[0], low, b[0], b[1]);
-        H::mma(d1[1], low, b[2], b[3]);
+        H::mma(d1[0], low, b[0], b[1], d1[0]);
+        H::mma(d1[1], low, b[2], b[3], d1[1]);
       }
     }
     float s[2][2];
@@ -344,9 +358,17 @@ struct PathMma {
     for (int n = 0; n < 2; n++)
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        const float x = d0[n][i] + (d0[n][2 + i] + (H::THREE ? d1[n][i] : 0.f));
-        s[n][i] = (ok >> (n * 8 + c + i)) & 1 ? (H::THREE ? x : x * unscale) : -INFINITY;
+        float x = d0[n][i] + (d0[n][2 + i] + (EXTRA ? d1[n][i] : 0.f));
+        if constexpr (SPLIT) x += __shfl_xor_sync(0xffffffffu, x, 16);
+        s[n][i] = H::THREE ? x : x * unscale;
       }
+    if (ok != 0xFFFF) {
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+          if (!((ok >> (n * 8 + c + i)) & 1)) s[n][i] = -INFINITY;
+    }
     float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -357,31 +379,22 @@ struct PathMma {
 #pragma unroll
       for (int j = 0; j < 2 * KD; j++) acc[j][0] *= f, acc[j][1] *= f;
     }
-    float p[2][2];
     uint32_t pa[4], pb[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int n = 0; n < 2; n++) {
-      p[n][0] = exp2_of(s[n][0], m);
-      p[n][1] = exp2_of(s[n][1], m);
-      l += p[n][0] + p[n][1];
-      pa[2 * n] = H::pack(p[n][0], p[n][1]);
-      const float2 f0 = H::unpack(pa[2 * n]);
-      const float u = p[n][0] - f0.x, v = p[n][1] - f0.y;
-      pa[2 * n + 1] = H::pack(u, v);
-      if constexpr (H::THREE) {
-        const float2 f1 = H::unpack(pa[2 * n + 1]);
-        pb[2 * n] = H::pack(u - f1.x, v - f1.y);
-      }
+      const float u = exp2_of(s[n][0], m), v = exp2_of(s[n][1], m);
+      l += u + v;
+      parts(u, v, pa[2 * n], pa[2 * n + 1], pb[2 * n]);
     }
 #pragma unroll
     for (int j = 0; j < KD; j++) {
       uint32_t b[4];
-      ldmatrix4_trans(b, vs + j * 32);
+      ldmatrix4_trans(b, vs + j / 4 * SLAB_BYTES + (((j % 4 * 2 + vu) ^ sw) << 4));
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        float d[4] = {};
-        H::mma(d, pa, b[2 * i], b[2 * i + 1]);
-        if constexpr (H::THREE) H::mma(d, pb, b[2 * i], b[2 * i + 1]);
+        float d[4];
+        H::mma(d, pa, b[2 * i], b[2 * i + 1], zero);
+        if constexpr (EXTRA) H::mma(d, pb, b[2 * i], b[2 * i + 1], d);
         acc[2 * j + i][0] += d[0] + d[2];
         acc[2 * j + i][1] += d[1] + d[3];
       }
@@ -389,17 +402,22 @@ struct PathMma {
   }
 
   __device__ void finish(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
-    const int lane = threadIdx.x & 31, r = lane >> 2, c = (lane & 3) * 2, dim = a.kv.dim;
+    const int r = row(), c = (threadIdx.x & 3) * 2, dim = a.kv.dim;
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     bool bad = !(fabsf(l) < INFINITY);
 #pragma unroll
-    for (int j = 0; j < 2 * KD; j++) bad |= !(fabsf(acc[j][0]) < INFINITY) || !(fabsf(acc[j][1]) < INFINITY);
+    for (int j = 0; j < 2 * KD; j++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        if constexpr (SPLIT) acc[j][i] += __shfl_xor_sync(0xffffffffu, acc[j][i], 16);
+        bad |= !(fabsf(acc[j][i]) < INFINITY);
+      }
     if (__any_sync(0xffffffffu, bad && r < a.part)) {
       attend_plain<T>(a, b, hc, j0, j1, rec);
       return;
     }
-    if (r < a.part) {
+    if (r < a.part && !(SPLIT && (threadIdx.x & 16))) {
       float* x = rec + r * (dim + 2);
       if (c == 0) {
         x[0] = m;
@@ -419,7 +437,7 @@ struct PathMma {
 // ------------------------------------------------------- fp32 caches (and wide 16-bit heads)
 //
 // LPR lanes share a row, each with CPL units of 16 bytes of it, so a warp treats 32 / LPR positions at
-// a time, R times per tile.  A lane copies exactly the units that it reads itself.  The R * GT partial
+// a time, R times per tile.  The R * GT partial
 // scores of a lane are summed over the lanes of a row by halving: each step exchanges half of the
 // values with a lane that keeps the other half, so 32 sums cost 31 shuffles and not 160, and each
 // lane ends with the scores that it turns into weights (no weight is computed twice).
@@ -427,10 +445,11 @@ template <typename T, int LPR, int CPL, int GT>
 struct PathFma {
   static constexpr int VE = 16 / (int)sizeof(T), KPW = 32 / LPR;
   static constexpr int KT = LPR <= 16 ? 16 : CPL == 1 ? 8 : 4, R = KT / KPW;
-  static constexpr int WARPS = 8, UNIT = VE;
-  static constexpr bool RING = true;
-  static constexpr int TILE_BYTES = 2 * R * CPL * 512;
-  static constexpr int STAGE_BYTES = TILE_BYTES + KT * GT * 4;
+  static constexpr int WARPS = 8;
+  static constexpr bool RING = true, SWIZZLE = false;
+  static constexpr int SLAB = LPR * CPL * VE, SLABS = 1, PITCH = SLAB * (int)sizeof(T), SLAB_BYTES = KT * PITCH;
+  static constexpr int TILE_BYTES = 2 * SLAB_BYTES;
+  static constexpr int STAGE_BYTES = TILE_BYTES + (KT * GT * 4 + 127) / 128 * 128;
   static constexpr int STAGES = TILE_BYTES >= 8192 ? 2 : 4;
   static constexpr int V = R * GT, NV = V > LPR ? V / LPR : 1;  // scores per lane
   static constexpr int SAME = LPR / GT;                         // lanes of a row with scores of one head
@@ -442,8 +461,6 @@ struct PathFma {
   __device__ static int lane_in() { return (threadIdx.x & 31) % LPR; }
   __device__ static int group() { return (threadIdx.x & 31) / LPR; }
   __device__ static int first() { return V >= LPR ? lane_in() * NV : lane_in() / COPIES; }  // score index g * R + r
-
-  __device__ void setup(const AttendArgs&, char*) {}
 
   __device__ void begin(const AttendArgs& a, int b, int hc) {
     const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * a.part, dim = a.kv.dim;
@@ -462,26 +479,10 @@ struct PathFma {
     l = 0.f;
   }
 
-  __device__ void issue(const AttendArgs& a, char* st, int lane, uint32_t row) {
-    const uint32_t dst = smem_u32(st) + lane * 16, units = a.kv.dim / VE;
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-      const uint32_t at = __shfl_sync(0xffffffffu, row, r * KPW + group());
-#pragma unroll
-      for (int c = 0; c < CPL; c++) {
-        const uint32_t u = lane_in() + c * LPR;
-        const bool live = at != kNoRow && u < units;
-        const size_t off = live ? ((size_t)at + u) << 4 : 0;
-        cp_async16(dst + (r * CPL + c) * 512, (const char*)a.kc + off, live ? 16 : 0);
-        cp_async16(dst + ((R + r) * CPL + c) * 512, (const char*)a.vc + off, live ? 16 : 0);
-      }
-    }
-  }
-
   static __device__ __forceinline__ void load(const char* at, float (&x)[CPL * VE]) {
 #pragma unroll
     for (int c = 0; c < CPL; c++) {
-      const uint4 u = *reinterpret_cast<const uint4*>(at + c * 512);
+      const uint4 u = *reinterpret_cast<const uint4*>(at + c * LPR * 16);
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -515,12 +516,12 @@ struct PathFma {
   }
 
   __device__ void tile(const AttendArgs&, char* st, uint32_t ok) {
-    const int lane = threadIdx.x & 31;
+    const char* rows = st + group() * PITCH + lane_in() * 16;
     float s[V];
 #pragma unroll
     for (int r = 0; r < R; r++) {
       float k[CPL * VE];
-      load(st + r * CPL * 512 + lane * 16, k);
+      load(rows + r * KPW * PITCH, k);
 #pragma unroll
       for (int g = 0; g < GT; g++) {
         float x = q[g][0] * k[0];
@@ -568,7 +569,7 @@ struct PathFma {
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         float v[CPL * VE];
-        load(st + (R + r4 + r) * CPL * 512 + lane * 16, v);
+        load(rows + (KT + (r4 + r) * KPW) * PITCH, v);
 #pragma unroll
         for (int g = 0; g < GT; g++)
 #pragma unroll
@@ -612,13 +613,16 @@ struct PathFma {
 // ------------------------------------------------------------------------------ the kernel
 template <typename P>
 constexpr size_t ring_bytes() {
-  return (size_t)P::WARPS * P::STAGES * (P::STAGE_BYTES + 16);
+  return (size_t)P::WARPS * P::STAGES * (P::STAGE_BYTES + 16);  // stages, then barriers and row bits of each
 }
 
 template <typename P>
-__global__ void __launch_bounds__(P::WARPS * 32) k_paged_attend(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(P::WARPS * 32)
+    k_paged_attend(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v) {
   constexpr int KT = P::KT, WARPS = P::WARPS, THREADS = WARPS * 32;
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ char smem_raw[];
+  char* smem = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;  // the swizzle's period
   __shared__ unsigned long long pre[kPrefix + 1];
   __shared__ unsigned long long warp_tot[WARPS];
   __shared__ long long seg_id[WARPS][2];  // first tile (on the line) of the sequence part in each record, -1: none
@@ -628,7 +632,17 @@ __global__ void __launch_bounds__(P::WARPS * 32) k_paged_attend(const __grid_con
   const int hcs = a.kv.kv_heads * a.chunks;
   const int rf = rec_floats(a);
   float* recs = reinterpret_cast<float*>(smem + ring_bytes<P>());
-  char* ring = smem + (size_t)w * P::STAGES * (P::STAGE_BYTES + 16);
+  char* ring = smem + w * P::STAGES * P::STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * P::STAGES * P::STAGE_BYTES) + w * P::STAGES * 2;  // barrier, bits
+  if constexpr (P::RING) {
+    if (tid == 0) {
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+    }
+    if (lane < P::STAGES) mbar_init(&bars[lane * 2], 1);
+    mbar_fence_init();
+    fence_async();
+  }
 
   // Tiles before every `step`-th sequence, for the whole batch.
   const int step = (a.kv.batch + kPrefix - 1) / kPrefix, n_pre = (a.kv.batch + step - 1) / step;
@@ -677,16 +691,16 @@ __global__ void __launch_bounds__(P::WARPS * 32) k_paged_attend(const __grid_con
   }
 
   // This block's stretch of the line, and this warp's.
-  const unsigned long long least = (unsigned long long)WARPS * a.min_tiles;
-  const unsigned long long want = (total + least - 1) / least;
+  const unsigned long long want = div64(total, WARPS * a.min_tiles) + 1;
   const unsigned blocks = want < gridDim.x ? (unsigned)want : gridDim.x;
-  if (blockIdx.x >= blocks) return;
-  const unsigned long long lo = total * blockIdx.x / blocks, hi = total * (blockIdx.x + 1) / blocks;
-  const unsigned long long wlo = lo + (hi - lo) * w / WARPS, whi = lo + (hi - lo) * (w + 1) / WARPS;
+  const unsigned long long share = div64(total + blocks - 1, blocks);  // tiles per block
+  const unsigned long long lo = share * blockIdx.x, hi = min(lo + share, total);
+  if (lo >= total) return;
+  const uint32_t each = ((uint32_t)(hi - lo) + WARPS - 1) / WARPS;
+  const unsigned long long wlo = min(lo + w * each, hi), whi = min(wlo + each, hi);
 
   if (wlo < whi) {
     P path;
-    path.setup(a, ring);
     Walk<KT> at;  // where the softmax is
     {
       int l = 0, r = n_pre - 1;
@@ -704,73 +718,103 @@ __global__ void __launch_bounds__(P::WARPS * 32) k_paged_attend(const __grid_con
         u += (unsigned long long)(s.t1 - s.t0) * hcs;
         s = seq_of<KT>(a, ++b);
       }
-      const unsigned long long in = wlo - u;
+      const uint32_t in = (uint32_t)(wlo - u);  // below 2^27 tiles times key heads of one sequence
       at.s = s;
       at.b = b;
       at.hc = (int)(in / (s.t1 - s.t0));
-      at.t = s.t0 + (uint32_t)(in % (s.t1 - s.t0));
+      at.t = s.t0 + in % (s.t1 - s.t0);
     }
     Walk<KT> ahead = at;  // where the copies are
-    const unsigned long long count = whi - wlo;
-    unsigned long long issued = 0;
-    // Page of this lane's row of the next tile to issue, fetched a tile early.
-    uint32_t id = kNoRow, slot = 0;
+    const uint32_t count = (uint32_t)(whi - wlo);
+    uint32_t issued = 0, stage_in = 0, stage_out = 0, parity = 0;
+    // Lane i looks up the page of the i-th box of the next tile to issue, a tile early.
+    const int boxes = a.page_tiles ? 1 : KT / a.box_rows;
+    uint32_t id = 0, slot = 0, span0 = 0, span1 = 0;
     bool live = false;
     auto look = [&]() {
-      const uint32_t j = ahead.t * KT + lane;
-      live = lane < KT && j >= ahead.s.first && j < ahead.s.n;
+      tile_span<KT>(a, ahead.t, &span0, &span1);
+      const uint32_t j = span0 + lane * a.box_rows;
+      live = lane < boxes && j < ahead.s.n && j + a.box_rows > ahead.s.first;
       const uint32_t pg = live ? page_of(a, j) : 0;
       slot = j - pg * a.kv.page_size;
-      id = live ? a.kv.table[(size_t)ahead.b * a.kv.max_pages + pg] : kNoRow;
+      id = live ? a.kv.table[(size_t)ahead.b * a.kv.max_pages + pg] : 0;
     };
     look();
     auto issue = [&]() {
       if (issued < count) {
-        uint32_t row = kNoRow;
-        if (live) {
-          if (id < a.kv.n_pages) {
-            if constexpr (P::RING)
-              row = (uint32_t)(((size_t)id * a.kv.page_stride + (size_t)(ahead.hc / a.chunks) * a.kv.head_stride +
-                                (size_t)slot * a.kv.slot_stride) /
-                               P::UNIT);
-            else
-              row = 0;
-          } else {
-            atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
-          }
-        }
-        const uint32_t ok = __ballot_sync(0xffffffffu, row != kNoRow);
-        char* st = ring + (issued % P::STAGES) * (P::STAGE_BYTES + 16);
+        const bool bad = live && id >= a.kv.n_pages;
+        if (bad) atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
         if constexpr (P::RING) {
-          if (lane == 0) *reinterpret_cast<uint32_t*>(st + P::STAGE_BYTES) = ok;
+          // rows that are attended to: within the sequence, the window and (one box only) the page
+          const uint32_t lo = ahead.s.first > span0 ? ahead.s.first - span0 : 0, hi = min(ahead.s.n, span1) - span0;
+          uint32_t ok = ((2u << (hi - 1)) - 1) & ~((1u << lo) - 1);
+          uint32_t lost = __ballot_sync(0xffffffffu, bad);
+          while (lost) {
+            const int x = __ffs(lost) - 1;
+            lost &= lost - 1;
+            ok &= ~(((1u << a.box_rows) - 1) << (x * a.box_rows));
+          }
+          char* st = ring + stage_in * P::STAGE_BYTES;
+          uint64_t* bar = &bars[stage_in * 2];
+          if (lane == 0) {
+            bar[1] = ok;
+            mbar_arrive_expect_tx(bar, 2 * P::SLABS * P::SLAB_BYTES);
+          }
+          __syncwarp();
+          if (lane < boxes) {
+            // a box without a page lies outside the tensor: zeros
+            const int page = live && !bad ? (int)id : (int)a.kv.n_pages, hk = ahead.hc / a.chunks;
+            const uint32_t dst = smem_u32(st) + lane * a.box_rows * (P::SLAB_BYTES / KT);
+#pragma unroll
+            for (int c = 0; c < P::SLABS; c++) {
+              tma_load_4d(dst + c * P::SLAB_BYTES, &tm_k, c * P::SLAB, (int)slot, hk, page, bar);
+              tma_load_4d(dst + (P::SLABS + c) * P::SLAB_BYTES, &tm_v, c * P::SLAB, (int)slot, hk, page, bar);
+            }
+          }
+          stage_in = stage_in + 1 == P::STAGES ? 0 : stage_in + 1;
         }
-        path.issue(a, st, lane, row);
         issued++;
         if (issued < count) {
           ahead.next(a, hcs);
           look();
         }
       }
-      if constexpr (P::RING) cp_commit();
     };
     for (int i = 0; i < P::STAGES - 1; i++) issue();
     uint32_t part_t = at.t;  // where this warp's share of the current sequence part begins
     path.begin(a, at.b, at.hc);
-    for (unsigned long long i = 0; i < count; i++) {
+    for (uint32_t i = 0; i < count; i++) {
       issue();
       if constexpr (P::RING) {
-        cp_wait<P::STAGES - 1>();
+        char* st = ring + stage_out * P::STAGE_BYTES;
+        mbar_wait(&bars[stage_out * 2], parity, a.flags, kWaitSite);
         __syncwarp();
-        char* st = ring + (i % P::STAGES) * (P::STAGE_BYTES + 16);
-        path.tile(a, st, *reinterpret_cast<uint32_t*>(st + P::STAGE_BYTES));
+        const uint32_t ok = (uint32_t)bars[stage_out * 2 + 1];
+        if (ok != (1u << KT) - 1) {
+          // what the cache holds behind a sequence's end may be NaN, and 0 * NaN is not 0
+          constexpr int ROW = P::SLAB_BYTES / KT;
+          for (int e = lane * 16; e < P::SLABS * P::SLAB_BYTES; e += 512)
+            if (!((ok >> (e % P::SLAB_BYTES / ROW)) & 1))
+              *reinterpret_cast<uint4*>(st + P::SLABS * P::SLAB_BYTES + e) = make_uint4(0, 0, 0, 0);
+          fence_async();
+          __syncwarp();
+        }
+        path.tile(a, st, ok);
         __syncwarp();
+        if (++stage_out == P::STAGES) {
+          stage_out = 0;
+          parity ^= 1;
+        }
       }
       const bool ends = at.t + 1 == at.s.t1;
       if (ends || i + 1 == count) {
         const bool starts = part_t == at.s.t0;
         const int which = starts ? 1 : 0;
         float* rec = recs + (w * 2 + which) * rf;
-        path.finish(a, at.b, at.hc, max(at.s.first, part_t * KT), min(at.s.n, (at.t + 1) * KT), rec);
+        uint32_t j0, j1, skip;
+        tile_span<KT>(a, part_t, &j0, &skip);
+        tile_span<KT>(a, at.t, &skip, &j1);
+        path.finish(a, at.b, at.hc, max(at.s.first, j0), min(at.s.n, j1), rec);
         if (starts && ends) {
           const int hk = at.hc / a.chunks, g0 = (at.hc - hk * a.chunks) * a.part;
           const int n_g = min(a.part, a.group - g0), h0 = hk * a.group + g0;
@@ -844,7 +888,7 @@ __global__ void __launch_bounds__(P::WARPS * 32) k_paged_attend(const __grid_con
     }
     if (before || behind) {
       // blocks that hold tiles u0 and u1 - 1
-      const int c0 = (int)(((u0 + 1) * blocks - 1) / total), c1 = (int)((u1 * blocks - 1) / total);
+      const int c0 = (int)div64(u0, share), c1 = (int)div64(u1 - 1, share);
       open_first[slot] = c0;
       open_parts[slot] = c1 - c0 + 1;
       open_b[slot] = b;
@@ -913,17 +957,57 @@ int sm_count(int device, int* out) {
   return OK;
 }
 
+// Tensor map of a paged cache: [page][head][slot][dim], boxes of `rows` slots x `cols` elements.
+int cache_map(CUtensorMap* map, const void* base, int dtype, const PagedLayout& kv, int cols, int rows, bool swizzle) {
+  const TensorMapEncode enc = tensor_map_encode();
+  if (!enc) {
+    set_error("cuTensorMapEncodeTiled entry point unavailable");
+    return ERR_CUDA;
+  }
+  const size_t es = cache_type_size(dtype);
+  cuuint64_t dims[4] = {(cuuint64_t)kv.dim, kv.page_size, (cuuint64_t)kv.kv_heads, kv.n_pages};
+  cuuint64_t strides[3] = {kv.slot_stride * es, kv.head_stride * es, kv.page_stride * es};
+  cuuint32_t box[4] = {(cuuint32_t)cols, (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map,
+                         dtype == TURT_CACHE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                         : dtype == TURT_CACHE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                         4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (code " + std::to_string((int)r) + ")");
+    return ERR_CUDA;
+  }
+  return OK;
+}
+
 template <typename P>
 int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
   static std::atomic<uint64_t> done{0};
   a.part = part;
   a.chunks = (a.group + part - 1) / part;
   a.min_tiles = 2;
+  a.box_rows = P::KT;
+  a.page_tiles = 0;
+  CUtensorMap tm_k{}, tm_v{};
+  if constexpr (P::RING) {
+    // a tile is one box, two half ones, or (page sizes that neither divides) what a page has of it
+    const int ps = (int)a.kv.page_size;
+    if (ps % P::KT != 0) {
+      if (P::KT >= 8 && ps % (P::KT / 2) == 0)
+        a.box_rows = P::KT / 2;
+      else
+        a.page_tiles = (ps + P::KT - 1) / P::KT;
+    }
+    RC(cache_map(&tm_k, a.kc, a.dtype, a.kv, P::SLAB, a.box_rows, P::SWIZZLE));
+    RC(cache_map(&tm_v, a.vc, a.dtype, a.kv, P::SLAB, a.box_rows, P::SWIZZLE));
+  }
   int sms = 0;
   RC(sm_count(ctx->device, &sms));
   const size_t rec = (size_t)P::WARPS * 2 * part * (a.kv.dim + 2) * 4;
   // the join of blocks keeps a weight per partial result and head
-  const size_t smem = std::max(ring_bytes<P>() + rec, (size_t)(kMaxBlocks + 1) * part * 4);
+  const size_t smem = std::max(ring_bytes<P>() + rec, (size_t)(kMaxBlocks + 1) * part * 4) + 1024;
   RC(smem_attr_per_device(done, k_paged_attend<P>, 218 * 1024));
   TURT_REQUIRE(smem <= 218 * 1024, "paged_attention: shared memory");
   static std::atomic<int> regs{0};
@@ -934,20 +1018,21 @@ int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
   }
   const int per_sm = smem <= 103 * 1024 && regs.load(std::memory_order_relaxed) <= 128 ? 2 : 1;
   const int grid = std::min(kMaxBlocks, sms * per_sm);
-  k_paged_attend<P><<<grid, P::WARPS * 32, smem, ctx->stream>>>(a);
+  k_paged_attend<P><<<grid, P::WARPS * 32, smem, ctx->stream>>>(a, tm_k, tm_v);
   TURT_LAUNCH_CHECK();
   return OK;
 }
 
-// Whether rows are whole 16-byte units on 16-byte boundaries whose numbers fit 32 bits.
+// Whether bulk tensor copies can read the cache: rows of whole 16-byte units on 16-byte boundaries, and
+// strides of which each divides the next larger one.
 template <typename T>
-bool in_units(const AttendArgs& a) {
+bool in_boxes(const AttendArgs& a) {
   const size_t n = 16 / sizeof(T);
   const PagedLayout& kv = a.kv;
-  const size_t last = (kv.n_pages - 1) * kv.page_stride + (kv.kv_heads - 1) * kv.head_stride +
-                      (kv.page_size - 1) * kv.slot_stride;
-  return aligned16(a.kc) && aligned16(a.vc) && kv.dim % n == 0 && kv.page_stride % n == 0 && kv.head_stride % n == 0 &&
-         kv.slot_stride % n == 0 && last / n < kNoRow;
+  size_t s[3] = {kv.slot_stride, kv.head_stride, kv.page_stride};
+  std::sort(s, s + 3);
+  return aligned16(a.kc) && aligned16(a.vc) && kv.dim % n == 0 && s[0] > 0 && s[0] % n == 0 && s[1] % s[0] == 0 &&
+         s[2] % s[1] == 0 && s[2] * sizeof(T) < ((size_t)1 << 40);
 }
 
 template <typename T, int LPR, int CPL, int MOST>
@@ -959,22 +1044,29 @@ int attend_fma(turt_ctx* ctx, const AttendArgs& a) {
   return ERR_UNSUPPORTED;
 }
 
+template <typename T, int KD>
+int attend_mma(turt_ctx* ctx, const AttendArgs& a) {
+  const int part = std::min(a.group, kGroup);
+  if constexpr (Half2<T>::THREE)
+    if (part <= 4) return attend_launch<PathMma<T, KD, true>>(ctx, a, part);
+  return attend_launch<PathMma<T, KD, false>>(ctx, a, part);
+}
+
 template <typename T>
 int attend_typed(turt_ctx* ctx, const AttendArgs& a) {
   const int dim = a.kv.dim;
-  if (!in_units<T>(a)) return attend_launch<PathPlain<T>>(ctx, a, 1);
+  if (!in_boxes<T>(a)) return attend_launch<PathPlain<T>>(ctx, a, 1);
   if constexpr (sizeof(T) == 4) {
     if (dim <= 32) return attend_fma<T, 8, 1, 8>(ctx, a);
     if (dim <= 64) return attend_fma<T, 16, 1, 8>(ctx, a);
     if (dim <= 128) return attend_fma<T, 32, 1, 8>(ctx, a);
     return attend_fma<T, 32, 2, 4>(ctx, a);
   } else {
-    const int part = std::min(a.group, kGroup);
-    if (dim <= 32) return attend_launch<PathMma<T, 2>>(ctx, a, part);
-    if (dim <= 64) return attend_launch<PathMma<T, 4>>(ctx, a, part);
-    if (dim <= 80) return attend_launch<PathMma<T, 5>>(ctx, a, part);
-    if (dim <= 96) return attend_launch<PathMma<T, 6>>(ctx, a, part);
-    if (dim <= 128) return attend_launch<PathMma<T, 8>>(ctx, a, part);
+    if (dim <= 32) return attend_mma<T, 2>(ctx, a);
+    if (dim <= 64) return attend_mma<T, 4>(ctx, a);
+    if (dim <= 80) return attend_mma<T, 5>(ctx, a);
+    if (dim <= 96) return attend_mma<T, 6>(ctx, a);
+    if (dim <= 128) return attend_mma<T, 8>(ctx, a);
     return attend_fma<T, 32, 1, 4>(ctx, a);
   }
 }
@@ -1028,6 +1120,7 @@ extern "C" int turt_paged_attention(turt_ctx* ctx, const turt_paged_kv* kv, cons
   a.counters = static_cast<uint32_t*>(workspace);
   a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
   a.flags = ctx->flags;
+  a.dtype = kv->dtype;
   if (kv->dtype == TURT_CACHE_F32) return attend_typed<float>(ctx, a);
   if (kv->dtype == TURT_CACHE_F16) return attend_typed<__half>(ctx, a);
   return attend_typed<__nv_bfloat16>(ctx, a);
