@@ -42,6 +42,7 @@ struct AttendArgs {
   uint32_t div_mul;  // position / page_size = position * div_mul >> div_shift (positions < 2^31)
   int div_shift;
   int min_tiles;     // tiles per warp, at least
+  int whole_tiles;   // tiles per warp up to which a block takes whole sequence parts
   int box_rows;      // positions per copy
   int page_tiles;    // tiles per page where tiles do not cross pages, 0: any KT positions are a tile
   uint32_t* counters;
@@ -621,12 +622,14 @@ __global__ void __launch_bounds__(P::WARPS * 32)
     k_paged_attend(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v) {
   constexpr int KT = P::KT, WARPS = P::WARPS, THREADS = WARPS * 32;
+  static_assert(2 * WARPS <= 32, "a lane per record");
   extern __shared__ char smem_raw[];
   char* smem = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;  // the swizzle's period
-  __shared__ unsigned long long pre[kPrefix + 1];
+  __shared__ unsigned long long pre[kPrefix];
   __shared__ unsigned long long warp_tot[WARPS];
-  __shared__ long long seg_id[WARPS][2];  // first tile (on the line) of the sequence part in each record, -1: none
-  __shared__ int seg_b[WARPS][2], seg_hc[WARPS][2];
+  __shared__ uint32_t warp_long[WARPS], warp_live[WARPS];
+  __shared__ long long seg_id[WARPS * 2];  // first tile (on the line) of the sequence part in each record, -1: none
+  __shared__ int seg_b[WARPS * 2], seg_hc[WARPS * 2];
   __shared__ unsigned s_old[2];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, dim = a.kv.dim;
   const int hcs = a.kv.kv_heads * a.chunks;
@@ -643,87 +646,108 @@ __global__ void __launch_bounds__(P::WARPS * 32)
     mbar_fence_init();
     fence_async();
   }
+  if (tid < WARPS * 2) seg_id[tid] = -1;
 
-  // Tiles before every `step`-th sequence, for the whole batch.
-  const int step = (a.kv.batch + kPrefix - 1) / kPrefix, n_pre = (a.kv.batch + step - 1) / step;
-  {
-    constexpr int PER = (kPrefix + THREADS - 1) / THREADS;
-    unsigned long long mine[PER], sum = 0;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int e = tid * PER + i;
-      mine[i] = sum;
-      if (e < n_pre)
-        for (int b = e * step; b < min(a.kv.batch, (e + 1) * step); b++) {
-          if (a.kv.lens[b] > a.kv.max_pages * a.kv.page_size && blockIdx.x == 0)
-            atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
-          const Seq s = seq_of<KT>(a, b);
-          sum += (unsigned long long)(s.t1 - s.t0) * hcs;
-        }
-    }
+  // Tiles before every `step`-th sequence, the longest part, and how many parts there are.
+  const int step = (a.kv.batch + kPrefix - 1) / kPrefix, n_pre = step == 1 ? a.kv.batch : (a.kv.batch + step - 1) / step;
+  unsigned long long total = 0;
+  uint32_t longest = 0, live_seqs = 0;
+  for (int e0 = 0; e0 < n_pre; e0 += THREADS) {
+    const int e = e0 + tid;
+    unsigned long long sum = 0;
+    uint32_t most = 0, live = 0;
+    if (e < n_pre)
+      for (int b = e * step; b < min(a.kv.batch, (e + 1) * step); b++) {
+        const Seq s = seq_of<KT>(a, b);
+        if (s.n == 0 && a.kv.lens[b] != 0 && blockIdx.x == 0) atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
+        sum += s.t1 - s.t0;
+        most = max(most, s.t1 - s.t0);
+        live += s.n != 0;
+      }
+    sum *= hcs;
     unsigned long long inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
-    if (lane == 31) warp_tot[w] = inc;
-    __syncthreads();
-    unsigned long long base = inc - sum;
-    for (int i = 0; i < w; i++) base += warp_tot[i];
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int e = tid * PER + i;
-      if (e < n_pre) pre[e] = base + mine[i];
+    most = __reduce_max_sync(0xffffffffu, most);
+    live = __reduce_add_sync(0xffffffffu, live);
+    if (lane == 31) {
+      warp_tot[w] = inc;
+      warp_long[w] = most;
+      warp_live[w] = live;
     }
-    if (tid == THREADS - 1) pre[n_pre] = base + sum;
+    __syncthreads();
+    unsigned long long before = total + inc - sum;
+#pragma unroll
+    for (int i = 0; i < WARPS; i++) {
+      const unsigned long long x = warp_tot[i];
+      if (i < w) before += x;
+      total += x;
+      longest = max(longest, warp_long[i]);
+      live_seqs += warp_live[i];
+    }
+    if (e < n_pre) pre[e] = before;
+    __syncthreads();
   }
-  if (tid < WARPS * 2) seg_id[tid >> 1][tid & 1] = -1;
-  __syncthreads();
-  const unsigned long long total = pre[n_pre];
 
   // Idle sequences: zeros.
-  for (int b = blockIdx.x; b < a.kv.batch; b += gridDim.x) {
-    if (seq_of<KT>(a, b).n) continue;
-    for (int e = tid; e < a.heads * dim; e += THREADS) a.out[(size_t)b * a.os + e] = 0.f;
-    if (a.lse)
-      for (int e = tid; e < a.heads; e += THREADS) a.lse[(size_t)b * a.heads + e] = -INFINITY;
-  }
+  if (live_seqs < (uint32_t)a.kv.batch)
+    for (int b = blockIdx.x; b < a.kv.batch; b += gridDim.x) {
+      if (seq_of<KT>(a, b).n) continue;
+      for (int e = tid; e < a.heads * dim; e += THREADS) a.out[(size_t)b * a.os + e] = 0.f;
+      if (a.lse)
+        for (int e = tid; e < a.heads; e += THREADS) a.lse[(size_t)b * a.heads + e] = -INFINITY;
+    }
+  if (total == 0) return;
 
-  // This block's stretch of the line, and this warp's.
-  const unsigned long long want = div64(total, WARPS * a.min_tiles) + 1;
+  // The place of tile u on the line, and the first tile of its sequence part.
+  auto locate = [&](unsigned long long u, Walk<KT>& at) -> unsigned long long {
+    int l = 0, r = n_pre - 1;
+    while (l < r) {
+      const int mid = (l + r + 1) >> 1;
+      if (pre[mid] <= u)
+        l = mid;
+      else
+        r = mid - 1;
+    }
+    unsigned long long x = pre[l];
+    at.b = l * step;
+    at.s = seq_of<KT>(a, at.b);
+    while (x + (unsigned long long)(at.s.t1 - at.s.t0) * hcs <= u) {
+      x += (unsigned long long)(at.s.t1 - at.s.t0) * hcs;
+      at.s = seq_of<KT>(a, ++at.b);
+    }
+    const uint32_t in = (uint32_t)(u - x), tiles = at.s.t1 - at.s.t0;  // below 2^27 tiles times key heads of one sequence
+    at.hc = (int)(in / tiles);
+    at.t = at.s.t0 + in - at.hc * tiles;
+    return u - (at.t - at.s.t0);
+  };
+
+  // This block's stretch of the line, and this warp's.  Where every part of a sequence is short, blocks
+  // take whole parts: the join between blocks costs more than the evenness gives.
+  const bool whole = longest <= WARPS * a.whole_tiles;
+  const unsigned long long want = whole ? (unsigned long long)live_seqs * hcs : div64(total, WARPS * a.min_tiles) + 1;
   const unsigned blocks = want < gridDim.x ? (unsigned)want : gridDim.x;
   const unsigned long long share = div64(total + blocks - 1, blocks);  // tiles per block
-  const unsigned long long lo = share * blockIdx.x, hi = min(lo + share, total);
+  unsigned long long lo = share * blockIdx.x, hi = min(lo + share, total);
   if (lo >= total) return;
+  if (whole) {  // the parts that begin in the stretch
+    Walk<KT> x;
+    unsigned long long s0 = locate(lo, x);
+    if (s0 != lo) lo = s0 + (x.s.t1 - x.s.t0);
+    s0 = locate(hi - 1, x);
+    hi = max(hi, s0 + (x.s.t1 - x.s.t0));
+    if (lo >= hi) return;
+  }
   const uint32_t each = ((uint32_t)(hi - lo) + WARPS - 1) / WARPS;
   const unsigned long long wlo = min(lo + w * each, hi), whi = min(wlo + each, hi);
 
   if (wlo < whi) {
     P path;
     Walk<KT> at;  // where the softmax is
-    {
-      int l = 0, r = n_pre - 1;
-      while (l < r) {
-        const int mid = (l + r + 1) >> 1;
-        if (pre[mid] <= wlo)
-          l = mid;
-        else
-          r = mid - 1;
-      }
-      unsigned long long u = pre[l];
-      int b = l * step;
-      Seq s = seq_of<KT>(a, b);
-      while (u + (unsigned long long)(s.t1 - s.t0) * hcs <= wlo) {
-        u += (unsigned long long)(s.t1 - s.t0) * hcs;
-        s = seq_of<KT>(a, ++b);
-      }
-      const uint32_t in = (uint32_t)(wlo - u);  // below 2^27 tiles times key heads of one sequence
-      at.s = s;
-      at.b = b;
-      at.hc = (int)(in / (s.t1 - s.t0));
-      at.t = s.t0 + in % (s.t1 - s.t0);
-    }
+    locate(wlo, at);
     Walk<KT> ahead = at;  // where the copies are
     const uint32_t count = (uint32_t)(whi - wlo);
     uint32_t issued = 0, stage_in = 0, stage_out = 0, parity = 0;
@@ -825,9 +849,9 @@ __global__ void __launch_bounds__(P::WARPS * 32)
           if (lane < n_g) store_lse(a, at.b, h0 + lane, rec[lane * (dim + 2)], rec[lane * (dim + 2) + 1]);
           __syncwarp();
         } else if (lane == 0) {
-          seg_id[w][which] = (long long)(wlo + i) - (long long)(at.t - at.s.t0);
-          seg_b[w][which] = at.b;
-          seg_hc[w][which] = at.hc;
+          seg_id[w * 2 + which] = (long long)(wlo + i) - (long long)(at.t - at.s.t0);
+          seg_b[w * 2 + which] = at.b;
+          seg_hc[w * 2 + which] = at.hc;
         }
         if (i + 1 < count) {
           at.next(a, hcs);
@@ -841,108 +865,124 @@ __global__ void __launch_bounds__(P::WARPS * 32)
   }
   __syncthreads();
 
-  // Join the warps' records, in the order of positions; records r = 2 w + which of one sequence part
-  // follow one another.  A part that lies in this block whole is done; the block's first may have
+  // Join the warps' records, in the order of positions.  Records r = 2 w + which of one sequence part
+  // follow one another; lane r holds record r's id, so every warp knows the runs.  A warp joins one
+  // head of one run at a time.  A part that lies in this block whole is done; the block's first may have
   // begun before it (slot 0), its last may go on behind it (slot 1).
-  int open_first[2] = {-1, -1}, open_b[2], open_hc[2], open_parts[2];
-  for (int r = 0; r < 2 * WARPS; r++) {
-    const long long id = seg_id[r >> 1][r & 1];
-    if (id < 0) continue;
-    int end = r + 1;
-    for (int e = r + 1; e < 2 * WARPS; e++) {
-      const long long x = seg_id[e >> 1][e & 1];
-      if (x >= 0 && x != id) break;
-      if (x == id) end = e + 1;
+  const long long my_id = lane < 2 * WARPS ? seg_id[lane] : -1;
+  const uint32_t used = __ballot_sync(0xffffffffu, my_id >= 0);
+  const uint32_t below = used & ((1u << lane) - 1);
+  const long long prev = __shfl_sync(0xffffffffu, my_id, below ? 31 - __clz(below) : 0);
+  const uint32_t heads_of_runs = __ballot_sync(0xffffffffu, my_id >= 0 && (!below || prev != my_id));
+  const int n_runs = __popc(heads_of_runs);
+  int open_first[2] = {-1, -1}, open_parts[2] = {0, 0}, open_rec[2] = {0, 0};
+  uint32_t left = heads_of_runs;
+  for (int run = 0, item = 0; run < n_runs; run++) {
+    const int r0 = __ffs(left) - 1;
+    left &= left - 1;
+    const uint32_t mine = used & (left ? (1u << (__ffs(left) - 1)) - 1 : 0xffffffffu) & ~((1u << r0) - 1);
+    const int b = seg_b[r0], hc = seg_hc[r0];
+    int hk = hc, g0 = 0;
+    if (a.chunks > 1) {
+      hk = hc / a.chunks;
+      g0 = (hc - hk * a.chunks) * a.part;
     }
-    const int b = seg_b[r >> 1][r & 1], hc = seg_hc[r >> 1][r & 1];
-    const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * a.part;
     const int n_g = min(a.part, a.group - g0), h0 = hk * a.group + g0;
-    const Seq s = seq_of<KT>(a, b);
-    const unsigned long long u0 = id, u1 = u0 + (s.t1 - s.t0);
-    const bool before = u0 < lo, behind = u1 > hi;
-    const int slot = before ? 0 : 1;
-    float* part = a.partial + (size_t)(blockIdx.x * 2 + slot) * rf;
-    for (int e = tid; e < n_g * dim; e += THREADS) {
-      const int g = e / dim, d = e - g * dim;
-      float top = -INFINITY;
-      for (int x = r; x < end; x++)
-        if (seg_id[x >> 1][x & 1] == id) top = fmaxf(top, recs[x * rf + g * (dim + 2)]);
-      float o = 0.f, l = 0.f;
-      for (int x = r; x < end; x++) {
-        if (seg_id[x >> 1][x & 1] != id) continue;
-        const float* rec = recs + x * rf + g * (dim + 2);
-        const float f = weight_of(rec[0], rec[1], top);
-        l += f * rec[1];
-        o += f * rec[2 + d];
-      }
+    bool before = false, behind = false;
+    if (run == 0 || run == n_runs - 1) {
+      const Seq s = seq_of<KT>(a, b);
+      const unsigned long long u0 = seg_id[r0], u1 = u0 + (s.t1 - s.t0);
+      before = u0 < lo;
+      behind = u1 > hi;
       if (before || behind) {
-        __stcg(part + g * (dim + 2) + 2 + d, o);
-        if (d == 0) {
-          __stcg(part + g * (dim + 2), top);
-          __stcg(part + g * (dim + 2) + 1, l);
-        }
-      } else {
-        store_out(a, b, h0 + g, d, o, l);
-        if (d == 0) store_lse(a, b, h0 + g, top, l);
+        // blocks that hold tiles u0 and u1 - 1
+        const int slot = before ? 0 : 1, c0 = (int)div64(u0, share), c1 = (int)div64(u1 - 1, share);
+        open_first[slot] = c0;
+        open_parts[slot] = c1 - c0 + 1;
+        open_rec[slot] = r0;
       }
     }
-    if (before || behind) {
-      // blocks that hold tiles u0 and u1 - 1
-      const int c0 = (int)div64(u0, share), c1 = (int)div64(u1 - 1, share);
-      open_first[slot] = c0;
-      open_parts[slot] = c1 - c0 + 1;
-      open_b[slot] = b;
-      open_hc[slot] = hc;
+    for (int g = 0; g < n_g; g++, item++) {
+      if (item % WARPS != w) continue;
+      const float* rec = recs + g * (dim + 2);
+      float m = -INFINITY, l = 0.f;
+      if ((mine >> lane) & 1) {
+        m = rec[lane * rf];
+        l = rec[lane * rf + 1];
+      }
+      const float top = warp_max(m), f = weight_of(m, l, top), sum = warp_sum(f * l);
+      float* part = a.partial + (size_t)(blockIdx.x * 2 + (before ? 0 : 1)) * rf + g * (dim + 2);
+      for (int d = lane; d < (dim + 31) / 32 * 32; d += 32) {
+        float o = 0.f;
+        for (uint32_t x = mine; x; x &= x - 1) {
+          const int r = __ffs(x) - 1;
+          o += __shfl_sync(0xffffffffu, f, r) * rec[r * rf + 2 + min(d, dim - 1)];
+        }
+        if (d < dim) {
+          if (before || behind)
+            __stcg(part + 2 + d, o);
+          else
+            store_out(a, b, h0 + g, d, o, sum);
+        }
+      }
+      if (lane == 0) {
+        if (before || behind) {
+          __stcg(part, top);
+          __stcg(part + 1, sum);
+        } else {
+          store_lse(a, b, h0 + g, top, sum);
+        }
+      }
     }
-    r = end - 1;
   }
   if (open_first[0] < 0 && open_first[1] < 0) return;
   __threadfence();
   __syncthreads();
-  if (tid == 0) {
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-      if (open_first[i] >= 0) s_old[i] = atomicAdd(&a.counters[open_first[i]], 1u);
+  if (tid < 2) {
+    const int c0 = tid ? open_first[1] : open_first[0];
+    if (c0 >= 0) s_old[tid] = atomicAdd(&a.counters[c0], 1u);
   }
   __syncthreads();
-  float* wt = reinterpret_cast<float*>(smem);  // [parts][heads of the part] weights, then the sums
-#pragma unroll
   for (int i = 0; i < 2; i++) {
-    if (open_first[i] < 0 || s_old[i] + 1 != (unsigned)open_parts[i]) continue;
+    const int c0 = i ? open_first[1] : open_first[0], parts = i ? open_parts[1] : open_parts[0];
+    if (c0 < 0 || s_old[i] + 1 != (unsigned)parts) continue;
     // the last of its blocks to arrive: every partial result is there
     __threadfence();
-    if (tid == 0) a.counters[open_first[i]] = 0;
-    const int c0 = open_first[i], parts = open_parts[i], b = open_b[i], hc = open_hc[i];
+    if (tid == 0) a.counters[c0] = 0;
+    const int r0 = i ? open_rec[1] : open_rec[0], b = seg_b[r0], hc = seg_hc[r0];
     const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * a.part;
     const int n_g = min(a.part, a.group - g0), h0 = hk * a.group + g0;
-    const float* p0 = a.partial + ((size_t)c0 * 2 + 1) * rf;  // block c0's slot 1, then slot 0 of the next ones
-    auto at = [&](int x) { return x == 0 ? p0 : a.partial + (size_t)(c0 + x) * 2 * rf; };
-    __syncthreads();
     for (int g = w; g < n_g; g += WARPS) {
-      float top = -INFINITY, sum = 0.f;
-      for (int x = lane; x < parts; x += 32) top = fmaxf(top, __ldcg(at(x) + g * (dim + 2)));
-      top = warp_max(top);
-      for (int x = lane; x < parts; x += 32) {
-        const float* p = at(x) + g * (dim + 2);
-        const float l = __ldcg(p + 1), f = weight_of(__ldcg(p), l, top);
-        wt[x * n_g + g] = f;
-        sum += f * l;
+      // block c0's slot 1, then slot 0 of the next ones
+      const float* p0 = a.partial + (size_t)c0 * 2 * rf + g * (dim + 2);
+      float o[8] = {}, top = -INFINITY, sum = 0.f;
+      for (int x0 = 0; x0 < parts; x0 += 32) {
+        const int n = min(32, parts - x0);
+        float m = -INFINITY, l = 0.f;
+        if (lane < n) {
+          const float* p = p0 + ((x0 + lane) * 2 + (x0 + lane == 0)) * rf;
+          m = __ldcg(p);
+          l = __ldcg(p + 1);
+        }
+        const float to = fmaxf(top, warp_max(m)), back = weight_of(top, sum, to), f = weight_of(m, l, to);
+        sum = sum * back + warp_sum(f * l);
+        top = to;
+#pragma unroll
+        for (int k = 0; k < 8; k++) o[k] *= back;
+#pragma unroll 4
+        for (int x = 0; x < n; x++) {
+          const float fx = __shfl_sync(0xffffffffu, f, x);
+          const float* p = p0 + ((x0 + x) * 2 + (x0 + x == 0)) * rf + 2;
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+            if (lane + 32 * k < dim) o[k] += fx * __ldcg(p + lane + 32 * k);
+        }
       }
-      sum = warp_sum(sum);
-      if (lane == 0) {
-        wt[parts * n_g + g] = sum;
-        store_lse(a, b, h0 + g, top, sum);
-      }
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (lane + 32 * k < dim) store_out(a, b, h0 + g, lane + 32 * k, o[k], sum);
+      if (lane == 0) store_lse(a, b, h0 + g, top, sum);
     }
-    __syncthreads();
-    for (int e = tid; e < n_g * dim; e += THREADS) {
-      const int g = e / dim, d = e - g * dim;
-      float o = 0.f;
-#pragma unroll 8
-      for (int x = 0; x < parts; x++) o += wt[x * n_g + g] * __ldcg(at(x) + g * (dim + 2) + 2 + d);
-      store_out(a, b, h0 + g, d, o, wt[parts * n_g + g]);
-    }
-    __syncthreads();
   }
 }
 
@@ -988,6 +1028,7 @@ int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
   a.part = part;
   a.chunks = (a.group + part - 1) / part;
   a.min_tiles = 2;
+  a.whole_tiles = 4;
   a.box_rows = P::KT;
   a.page_tiles = 0;
   CUtensorMap tm_k{}, tm_v{};
@@ -1005,9 +1046,7 @@ int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
   }
   int sms = 0;
   RC(sm_count(ctx->device, &sms));
-  const size_t rec = (size_t)P::WARPS * 2 * part * (a.kv.dim + 2) * 4;
-  // the join of blocks keeps a weight per partial result and head
-  const size_t smem = std::max(ring_bytes<P>() + rec, (size_t)(kMaxBlocks + 1) * part * 4) + 1024;
+  const size_t rec = (size_t)P::WARPS * 2 * part * (a.kv.dim + 2) * 4, smem = ring_bytes<P>() + rec + 1024;
   RC(smem_attr_per_device(done, k_paged_attend<P>, 218 * 1024));
   TURT_REQUIRE(smem <= 218 * 1024, "paged_attention: shared memory");
   static std::atomic<int> regs{0};
