@@ -123,6 +123,8 @@ __global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ Ap
   __shared__ size_t s_off;
   __shared__ int s_pos, s_live;
   const int i = blockIdx.x;
+  pdl_wait();
+  pdl_trigger();
   if (threadIdx.x == 0) {
     int pos = 0;
     size_t off = 0;
@@ -201,10 +203,7 @@ __global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ Ap
 
 template <typename T>
 int append_launch(cudaStream_t st, const AppendArgs& a, bool vec) {
-  if (vec)
-    k_paged_append<T, 8><<<a.rows, 256, 0, st>>>(a);
-  else
-    k_paged_append<T, 2><<<a.rows, 256, 0, st>>>(a);
+  TURT_CHECK_CUDA(launch_pdl(vec ? k_paged_append<T, 8> : k_paged_append<T, 2>, dim3(a.rows), dim3(256), 0, st, a));
   TURT_LAUNCH_CHECK();
   return OK;
 }

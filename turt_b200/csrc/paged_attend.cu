@@ -49,6 +49,7 @@ struct AttendArgs {
   float* partial;
   int* flags;
   int dtype;
+  bool q_pairs;  // the elements of q can be read two at a time
 };
 
 __device__ __forceinline__ uint32_t page_of(const AttendArgs& a, uint32_t j) {
@@ -120,10 +121,23 @@ struct Walk {
 };
 
 // A result of part of a sequence: per head m (log2), l and dim unnormalised outputs.
-__device__ __forceinline__ int rec_floats(const AttendArgs& a) { return a.part * (a.kv.dim + 2); }
+__host__ __device__ __forceinline__ int rec_floats(int part, int dim) { return (part * (dim + 2) + 3) & ~3; }
 
 __device__ __forceinline__ float weight_of(float m, float l, float top) {
   return m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
+}
+
+// The heads of part hc of the head groups: kv head, first query head, how many.
+struct HeadPart {
+  int kv, head, n;
+};
+__device__ __forceinline__ HeadPart head_part(const AttendArgs& a, int hc) {
+  int kv = hc, g0 = 0;
+  if (a.chunks > 1) {
+    kv = hc / a.chunks;
+    g0 = (hc - kv * a.chunks) * a.part;
+  }
+  return {kv, kv * a.group + g0, min(a.part, a.group - g0)};
 }
 
 __device__ __forceinline__ void store_out(const AttendArgs& a, int b, int head, int d, float o, float l) {
@@ -133,6 +147,14 @@ __device__ __forceinline__ void store_lse(const AttendArgs& a, int b, int head, 
   if (a.lse) a.lse[(size_t)b * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
+// One head's outputs, element lane + 32 k in o[k].
+__device__ __forceinline__ void store_head(const AttendArgs& a, int b, int head, int lane, const float (&o)[8], float m, float l) {
+#pragma unroll
+  for (int k = 0; k < 8; k++)
+    if (lane + 32 * k < a.kv.dim) store_out(a, b, head, lane + 32 * k, o[k], l);
+  if (lane == 0) store_lse(a, b, head, m, l);
+}
+
 // One warp, any layout, head by head: positions [j0, j1) of sequence b into rec (one record of
 // a.part heads).  Lanes take every 32nd element.  The formula as it stands: also what a stretch
 // with infinities or NaN falls back to.
@@ -140,11 +162,11 @@ template <typename T>
 __device__ __noinline__ void attend_plain(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
   const PagedLayout& kv = a.kv;
   const int lane = threadIdx.x & 31, dim = kv.dim;
-  const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * a.part;
+  const HeadPart hp = head_part(a, hc);
   for (int g = 0; g < a.part; g++) {
     float q[8], o[8], m = -INFINITY, l = 0.f;
-    const float* qh = a.q + (size_t)b * a.qs + (size_t)(hk * a.group + g0 + g) * dim;
-    const bool head = g0 + g < a.group;
+    const float* qh = a.q + (size_t)b * a.qs + (size_t)(hp.head + g) * dim;
+    const bool head = g < hp.n;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       q[i] = head && lane + 32 * i < dim ? qh[lane + 32 * i] * a.scale : 0.f;
@@ -153,7 +175,7 @@ __device__ __noinline__ void attend_plain(const AttendArgs& a, int b, int hc, ui
     for (uint32_t j = j0; head && j < j1; j++) {
       const uint32_t pg = page_of(a, j), id = kv.table[(size_t)b * kv.max_pages + pg];
       if (id >= kv.n_pages) continue;  // flagged where the tile was opened
-      const size_t off = (size_t)id * kv.page_stride + (size_t)hk * kv.head_stride +
+      const size_t off = (size_t)id * kv.page_stride + (size_t)hp.kv * kv.head_stride +
                          (size_t)(j - pg * kv.page_size) * kv.slot_stride;
       const T *kr = (const T*)a.kc + off, *vr = (const T*)a.vc + off;
       float s = 0.f;
@@ -297,16 +319,26 @@ struct PathMma {
 
   __device__ void begin(const AttendArgs& a, int b, int hc) {
     const int r = row(), c = (threadIdx.x & 3) * 2, dim = a.kv.dim;
-    const int hk = hc / a.chunks, g = (hc - hk * a.chunks) * a.part + r;
-    const bool head = r < a.part && g < a.group;
-    const float* q = a.q + (size_t)b * a.qs + (size_t)(hk * a.group + (head ? g : 0)) * dim;
+    const HeadPart hp = head_part(a, hc);
+    const float* q = a.q + (size_t)b * a.qs + (size_t)(hp.head + (r < hp.n ? r : 0)) * dim + c;
     float x[KD][4], top = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2 * KD; k++) {
+      float2 y = make_float2(0.f, 0.f);
+      if (r < hp.n && k * 8 < dim) {
+        if (a.q_pairs)
+          y = *reinterpret_cast<const float2*>(q + k * 8);
+        else
+          y = make_float2(q[k * 8], q[k * 8 + 1]);
+      }
+      x[k >> 1][(k & 1) * 2] = y.x;
+      x[k >> 1][(k & 1) * 2 + 1] = y.y;
+    }
 #pragma unroll
     for (int k = 0; k < KD; k++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int d = k * 16 + (i >> 1) * 8 + c + (i & 1);
-        x[k][i] = head && d < dim ? q[d] * a.scale : 0.f;
+        x[k][i] *= a.scale;
         top = fmaxf(top, fabsf(x[k][i]));
       }
     float up = 1.f;
@@ -464,11 +496,12 @@ struct PathFma {
   __device__ static int first() { return V >= LPR ? lane_in() * NV : lane_in() / COPIES; }  // score index g * R + r
 
   __device__ void begin(const AttendArgs& a, int b, int hc) {
-    const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * a.part, dim = a.kv.dim;
+    const HeadPart hp = head_part(a, hc);
+    const int dim = a.kv.dim;
 #pragma unroll
     for (int g = 0; g < GT; g++) {
-      const bool head = g < a.part && g0 + g < a.group;
-      const float* x = a.q + (size_t)b * a.qs + (size_t)(hk * a.group + (head ? g0 + g : 0)) * dim;
+      const bool head = g < hp.n;
+      const float* x = a.q + (size_t)b * a.qs + (size_t)(hp.head + (head ? g : 0)) * dim;
 #pragma unroll
       for (int i = 0; i < CPL * VE; i++) {
         const int d = (lane_in() + (i / VE) * LPR) * VE + i % VE;
@@ -629,11 +662,12 @@ __global__ void __launch_bounds__(P::WARPS * 32)
   __shared__ unsigned long long warp_tot[WARPS];
   __shared__ uint32_t warp_long[WARPS], warp_live[WARPS];
   __shared__ long long seg_id[WARPS * 2];  // first tile (on the line) of the sequence part in each record, -1: none
-  __shared__ int seg_b[WARPS * 2], seg_hc[WARPS * 2];
+  __shared__ int seg_b[WARPS * 2], seg_hc[WARPS * 2], seg_tiles[WARPS * 2];
+  __shared__ int open_first[2], open_parts[2], open_rec[2];  // parts that other blocks share: first block, blocks, record
   __shared__ unsigned s_old[2];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, dim = a.kv.dim;
   const int hcs = a.kv.kv_heads * a.chunks;
-  const int rf = rec_floats(a);
+  const int rf = rec_floats(a.part, dim);
   float* recs = reinterpret_cast<float*>(smem + ring_bytes<P>());
   char* ring = smem + w * P::STAGES * P::STAGE_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * P::STAGES * P::STAGE_BYTES) + w * P::STAGES * 2;  // barrier, bits
@@ -647,6 +681,9 @@ __global__ void __launch_bounds__(P::WARPS * 32)
     fence_async();
   }
   if (tid < WARPS * 2) seg_id[tid] = -1;
+  if (tid < 2) open_first[tid] = -1;
+  pdl_wait();
+  pdl_trigger();
 
   // Tiles before every `step`-th sequence, the longest part, and how many parts there are.
   const int step = (a.kv.batch + kPrefix - 1) / kPrefix, n_pre = step == 1 ? a.kv.batch : (a.kv.batch + step - 1) / step;
@@ -715,7 +752,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
     unsigned long long x = pre[l];
     at.b = l * step;
     at.s = seq_of<KT>(a, at.b);
-    while (x + (unsigned long long)(at.s.t1 - at.s.t0) * hcs <= u) {
+    while (x + (unsigned long long)(at.s.t1 - at.s.t0) * hcs <= u && at.b + 1 < a.kv.batch) {
       x += (unsigned long long)(at.s.t1 - at.s.t0) * hcs;
       at.s = seq_of<KT>(a, ++at.b);
     }
@@ -787,7 +824,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
           __syncwarp();
           if (lane < boxes) {
             // a box without a page lies outside the tensor: zeros
-            const int page = live && !bad ? (int)id : (int)a.kv.n_pages, hk = ahead.hc / a.chunks;
+            const int page = live && !bad ? (int)id : (int)a.kv.n_pages, hk = head_part(a, ahead.hc).kv;
             const uint32_t dst = smem_u32(st) + lane * a.box_rows * (P::SLAB_BYTES / KT);
 #pragma unroll
             for (int c = 0; c < P::SLABS; c++) {
@@ -840,18 +877,18 @@ __global__ void __launch_bounds__(P::WARPS * 32)
         tile_span<KT>(a, at.t, &skip, &j1);
         path.finish(a, at.b, at.hc, max(at.s.first, j0), min(at.s.n, j1), rec);
         if (starts && ends) {
-          const int hk = at.hc / a.chunks, g0 = (at.hc - hk * a.chunks) * a.part;
-          const int n_g = min(a.part, a.group - g0), h0 = hk * a.group + g0;
-          for (int e = lane; e < n_g * dim; e += 32) {
-            const int g = e / dim, d = e - g * dim;
-            store_out(a, at.b, h0 + g, d, rec[g * (dim + 2) + 2 + d], rec[g * (dim + 2) + 1]);
+          const HeadPart hp = head_part(a, at.hc);
+          for (int g = 0; g < hp.n; g++) {
+            const float* x = rec + g * (dim + 2);
+            for (int d = lane; d < dim; d += 32) store_out(a, at.b, hp.head + g, d, x[2 + d], x[1]);
+            if (lane == 0) store_lse(a, at.b, hp.head + g, x[0], x[1]);
           }
-          if (lane < n_g) store_lse(a, at.b, h0 + lane, rec[lane * (dim + 2)], rec[lane * (dim + 2) + 1]);
           __syncwarp();
         } else if (lane == 0) {
           seg_id[w * 2 + which] = (long long)(wlo + i) - (long long)(at.t - at.s.t0);
           seg_b[w * 2 + which] = at.b;
           seg_hc[w * 2 + which] = at.hc;
+          seg_tiles[w * 2 + which] = at.s.t1 - at.s.t0;
         }
         if (i + 1 < count) {
           at.next(a, hcs);
@@ -873,116 +910,103 @@ __global__ void __launch_bounds__(P::WARPS * 32)
   const uint32_t used = __ballot_sync(0xffffffffu, my_id >= 0);
   const uint32_t below = used & ((1u << lane) - 1);
   const long long prev = __shfl_sync(0xffffffffu, my_id, below ? 31 - __clz(below) : 0);
-  const uint32_t heads_of_runs = __ballot_sync(0xffffffffu, my_id >= 0 && (!below || prev != my_id));
-  const int n_runs = __popc(heads_of_runs);
-  int open_first[2] = {-1, -1}, open_parts[2] = {0, 0}, open_rec[2] = {0, 0};
-  uint32_t left = heads_of_runs;
-  for (int run = 0, item = 0; run < n_runs; run++) {
+  uint32_t left = __ballot_sync(0xffffffffu, my_id >= 0 && (!below || prev != my_id));
+  bool any_open = false;
+  for (int item = 0; left;) {
     const int r0 = __ffs(left) - 1;
     left &= left - 1;
     const uint32_t mine = used & (left ? (1u << (__ffs(left) - 1)) - 1 : 0xffffffffu) & ~((1u << r0) - 1);
-    const int b = seg_b[r0], hc = seg_hc[r0];
-    int hk = hc, g0 = 0;
-    if (a.chunks > 1) {
-      hk = hc / a.chunks;
-      g0 = (hc - hk * a.chunks) * a.part;
+    const HeadPart hp = head_part(a, seg_hc[r0]);
+    const unsigned long long u0 = seg_id[r0], u1 = u0 + seg_tiles[r0];
+    const bool before = u0 < lo, open = before || u1 > hi;
+    any_open |= open;
+    if (open && tid == 0) {
+      // blocks that hold tiles u0 and u1 - 1
+      const int slot = before ? 0 : 1, c0 = (int)div64(u0, share);
+      open_first[slot] = c0;
+      open_parts[slot] = (int)div64(u1 - 1, share) - c0 + 1;
+      open_rec[slot] = r0;
     }
-    const int n_g = min(a.part, a.group - g0), h0 = hk * a.group + g0;
-    bool before = false, behind = false;
-    if (run == 0 || run == n_runs - 1) {
-      const Seq s = seq_of<KT>(a, b);
-      const unsigned long long u0 = seg_id[r0], u1 = u0 + (s.t1 - s.t0);
-      before = u0 < lo;
-      behind = u1 > hi;
-      if (before || behind) {
-        // blocks that hold tiles u0 and u1 - 1
-        const int slot = before ? 0 : 1, c0 = (int)div64(u0, share), c1 = (int)div64(u1 - 1, share);
-        open_first[slot] = c0;
-        open_parts[slot] = c1 - c0 + 1;
-        open_rec[slot] = r0;
-      }
-    }
-    for (int g = 0; g < n_g; g++, item++) {
+    for (int g = 0; g < hp.n; g++, item++) {
       if (item % WARPS != w) continue;
       const float* rec = recs + g * (dim + 2);
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f, o[8] = {};
       if ((mine >> lane) & 1) {
         m = rec[lane * rf];
         l = rec[lane * rf + 1];
       }
       const float top = warp_max(m), f = weight_of(m, l, top), sum = warp_sum(f * l);
-      float* part = a.partial + (size_t)(blockIdx.x * 2 + (before ? 0 : 1)) * rf + g * (dim + 2);
-      for (int d = lane; d < (dim + 31) / 32 * 32; d += 32) {
-        float o = 0.f;
-        for (uint32_t x = mine; x; x &= x - 1) {
-          const int r = __ffs(x) - 1;
-          o += __shfl_sync(0xffffffffu, f, r) * rec[r * rf + 2 + min(d, dim - 1)];
-        }
-        if (d < dim) {
-          if (before || behind)
-            __stcg(part + 2 + d, o);
-          else
-            store_out(a, b, h0 + g, d, o, sum);
-        }
+      for (uint32_t x = mine; x; x &= x - 1) {
+        const int r = __ffs(x) - 1;
+        const float fx = __shfl_sync(0xffffffffu, f, r), *p = rec + r * rf + 2 + lane;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (lane + 32 * k < dim) o[k] += fx * p[32 * k];
       }
-      if (lane == 0) {
-        if (before || behind) {
+      if (open) {
+        float* part = a.partial + (size_t)(blockIdx.x * 2 + (before ? 0 : 1)) * rf + g * (dim + 2);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (lane + 32 * k < dim) __stcg(part + 2 + lane + 32 * k, o[k]);
+        if (lane == 0) {
           __stcg(part, top);
           __stcg(part + 1, sum);
-        } else {
-          store_lse(a, b, h0 + g, top, sum);
         }
+      } else {
+        store_head(a, seg_b[r0], hp.head + g, lane, o, top, sum);
       }
     }
   }
-  if (open_first[0] < 0 && open_first[1] < 0) return;
+  if (!any_open) return;
   __threadfence();
   __syncthreads();
-  if (tid < 2) {
-    const int c0 = tid ? open_first[1] : open_first[0];
-    if (c0 >= 0) s_old[tid] = atomicAdd(&a.counters[c0], 1u);
-  }
+  if (tid < 2 && open_first[tid] >= 0) s_old[tid] = atomicAdd(&a.counters[open_first[tid]], 1u);
   __syncthreads();
   for (int i = 0; i < 2; i++) {
-    const int c0 = i ? open_first[1] : open_first[0], parts = i ? open_parts[1] : open_parts[0];
+    const int c0 = open_first[i], parts = open_parts[i];
     if (c0 < 0 || s_old[i] + 1 != (unsigned)parts) continue;
     // the last of its blocks to arrive: every partial result is there
     __threadfence();
     if (tid == 0) a.counters[c0] = 0;
-    const int r0 = i ? open_rec[1] : open_rec[0], b = seg_b[r0], hc = seg_hc[r0];
-    const int hk = hc / a.chunks, g0 = (hc - hk * a.chunks) * a.part;
-    const int n_g = min(a.part, a.group - g0), h0 = hk * a.group + g0;
-    for (int g = w; g < n_g; g += WARPS) {
-      // block c0's slot 1, then slot 0 of the next ones
-      const float* p0 = a.partial + (size_t)c0 * 2 * rf + g * (dim + 2);
-      float o[8] = {}, top = -INFINITY, sum = 0.f;
-      for (int x0 = 0; x0 < parts; x0 += 32) {
-        const int n = min(32, parts - x0);
-        float m = -INFINITY, l = 0.f;
-        if (lane < n) {
-          const float* p = p0 + ((x0 + lane) * 2 + (x0 + lane == 0)) * rf;
-          m = __ldcg(p);
-          l = __ldcg(p + 1);
-        }
-        const float to = fmaxf(top, warp_max(m)), back = weight_of(top, sum, to), f = weight_of(m, l, to);
-        sum = sum * back + warp_sum(f * l);
-        top = to;
+    const HeadPart hp = head_part(a, seg_hc[open_rec[i]]);
+    // Block c0's slot 1, then slot 0 of the next ones, brought to shared memory: one trip to L2 for
+    // all of them where they fit.
+    float* stage = reinterpret_cast<float*>(smem);
+    const int rf4 = rf / 4, most = 2 * WARPS + (int)(ring_bytes<P>() / 4) / rf;  // the ring, and the records behind it
+    float o[8] = {}, top = -INFINITY, sum = 0.f;  // of head w
+    for (int x0 = 0; x0 < parts; x0 += most) {
+      const int n = min(most, parts - x0);
+      __syncthreads();
+#pragma unroll 8
+      for (int e = tid; e < n * rf4; e += THREADS) {
+        const int x = e / rf4, at = (c0 + x0 + x) * 2 + (x0 + x == 0);
+        reinterpret_cast<float4*>(stage)[e] = __ldcg(reinterpret_cast<const float4*>(a.partial + (size_t)at * rf) + e - x * rf4);
+      }
+      __syncthreads();
+      if (w < hp.n) {
+        const float* rec = stage + w * (dim + 2);
+        for (int y0 = 0; y0 < n; y0 += 32) {
+          const int ny = min(32, n - y0);
+          float m = -INFINITY, l = 0.f;
+          if (lane < ny) {
+            m = rec[(y0 + lane) * rf];
+            l = rec[(y0 + lane) * rf + 1];
+          }
+          const float to = fmaxf(top, warp_max(m)), back = weight_of(top, sum, to), f = weight_of(m, l, to);
+          sum = sum * back + warp_sum(f * l);
+          top = to;
 #pragma unroll
-        for (int k = 0; k < 8; k++) o[k] *= back;
-#pragma unroll 4
-        for (int x = 0; x < n; x++) {
-          const float fx = __shfl_sync(0xffffffffu, f, x);
-          const float* p = p0 + ((x0 + x) * 2 + (x0 + x == 0)) * rf + 2;
+          for (int k = 0; k < 8; k++) o[k] *= back;
+          for (int y = 0; y < ny; y++) {
+            const float fx = __shfl_sync(0xffffffffu, f, y), *p = rec + (y0 + y) * rf + 2 + lane;
 #pragma unroll
-          for (int k = 0; k < 8; k++)
-            if (lane + 32 * k < dim) o[k] += fx * __ldcg(p + lane + 32 * k);
+            for (int k = 0; k < 8; k++)
+              if (lane + 32 * k < dim) o[k] += fx * p[32 * k];
+          }
         }
       }
-#pragma unroll
-      for (int k = 0; k < 8; k++)
-        if (lane + 32 * k < dim) store_out(a, b, h0 + g, lane + 32 * k, o[k], sum);
-      if (lane == 0) store_lse(a, b, h0 + g, top, sum);
     }
+    if (w < hp.n) store_head(a, seg_b[open_rec[i]], hp.head + w, lane, o, top, sum);
   }
 }
 
@@ -1046,7 +1070,7 @@ int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
   }
   int sms = 0;
   RC(sm_count(ctx->device, &sms));
-  const size_t rec = (size_t)P::WARPS * 2 * part * (a.kv.dim + 2) * 4, smem = ring_bytes<P>() + rec + 1024;
+  const size_t rec = (size_t)P::WARPS * 2 * rec_floats(part, a.kv.dim) * 4, smem = ring_bytes<P>() + rec + 1024;
   RC(smem_attr_per_device(done, k_paged_attend<P>, 218 * 1024));
   TURT_REQUIRE(smem <= 218 * 1024, "paged_attention: shared memory");
   static std::atomic<int> regs{0};
@@ -1057,7 +1081,7 @@ int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
   }
   const int per_sm = smem <= 103 * 1024 && regs.load(std::memory_order_relaxed) <= 128 ? 2 : 1;
   const int grid = std::min(kMaxBlocks, sms * per_sm);
-  k_paged_attend<P><<<grid, P::WARPS * 32, smem, ctx->stream>>>(a, tm_k, tm_v);
+  TURT_CHECK_CUDA(launch_pdl(k_paged_attend<P>, dim3(grid), dim3(P::WARPS * 32), smem, ctx->stream, a, tm_k, tm_v));
   TURT_LAUNCH_CHECK();
   return OK;
 }
@@ -1123,7 +1147,7 @@ extern "C" int turt_paged_attention_workspace(const turt_paged_kv* kv, int n_hea
   TURT_REQUIRE(bytes, "paged_attention_workspace: null bytes");
   TURT_REQUIRE(n_head > 0 && n_head % kv->n_kv_head == 0, "paged_attention: n_head must be a multiple of n_kv_head");
   const int part = std::min(kGroup, n_head / kv->n_kv_head);
-  *bytes = kCounterBytes + (size_t)kMaxBlocks * 2 * part * (kv->head_dim + 2) * 4;
+  *bytes = kCounterBytes + (size_t)kMaxBlocks * 2 * rec_floats(part, kv->head_dim) * 4;
   return OK;
 }
 
@@ -1160,6 +1184,7 @@ extern "C" int turt_paged_attention(turt_ctx* ctx, const turt_paged_kv* kv, cons
   a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
   a.flags = ctx->flags;
   a.dtype = kv->dtype;
+  a.q_pairs = (uintptr_t)q % 8 == 0 && q_stride % 2 == 0;
   if (kv->dtype == TURT_CACHE_F32) return attend_typed<float>(ctx, a);
   if (kv->dtype == TURT_CACHE_F16) return attend_typed<__half>(ctx, a);
   return attend_typed<__nv_bfloat16>(ctx, a);

@@ -58,6 +58,8 @@ __global__ void __launch_bounds__(kRuleThreads) k_logit_rules(const __grid_const
   const int s0 = blockIdx.x * a.slice - lead;  // id of the slice's first position (may be negative)
   const bool first = blockIdx.x == 0;
   if (s0 >= V) return;
+  pdl_wait();
+  pdl_trigger();
   const bool hist = a.r.tokens != nullptr, biased = a.r.bias_ids != nullptr;
   if (hist)
     for (int e = threadIdx.x * 4; e < a.slice; e += kRuleThreads * 4) *reinterpret_cast<uint4*>(cnt + e) = make_uint4(0, 0, 0, 0);
@@ -179,10 +181,7 @@ extern "C" int turt_logit_rules_apply(turt_ctx* ctx, const float* logits, size_t
   const bool vec = ((uintptr_t)logits & 15) == ((uintptr_t)out & 15) && (rows == 1 || ld % 4 == out_ld % 4);
   const size_t smem = (size_t)a.slice * 8;
   const dim3 grid(ceil_div((long)vocab + 3, a.slice), rows);
-  if (vec)
-    k_logit_rules<true><<<grid, kRuleThreads, smem, ctx->stream>>>(a);
-  else
-    k_logit_rules<false><<<grid, kRuleThreads, smem, ctx->stream>>>(a);
+  TURT_CHECK_CUDA(launch_pdl(vec ? k_logit_rules<true> : k_logit_rules<false>, grid, dim3(kRuleThreads), smem, ctx->stream, a));
   TURT_LAUNCH_CHECK();
   return OK;
 }
