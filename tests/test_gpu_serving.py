@@ -540,8 +540,41 @@ def test_rules(eng, rows, vocab):
     dict(penalties=("presence",)), dict(penalties=()), dict(pad=3), dict(pad=4, out_pad=8), dict(pad=4, out_pad=5),
     dict(shift=1), dict(shift=3, pad=2, masks="rows", biases=5), dict(in_place=True, biases=5, masks="rows"),
     dict(special=True, biases=5, masks="rows")])
-def test_rules_variants(eng, kw):
-    check_rules(eng, 6, 10007, seed=4, **kw)
+@pytest.mark.parametrize("rows,vocab", [(6, 10007), (310, 17001)])
+def test_rules_variants(eng, kw, rows, vocab):
+    """A few rows, and enough of them for the kernel of large batches (310 x 17001: three slices a row)."""
+    check_rules(eng, rows, vocab, seed=4, **kw)
+
+
+@pytest.mark.parametrize("rows,vocab", [(700, 7), (650, 8191), (601, 8192), (599, 8193), (300, 16385)])
+def test_rules_of_large_batches(eng, rows, vocab):
+    check_rules(eng, rows, vocab, seed=6, hist=(50, 30), biases=5, masks="rows")
+
+
+def test_rules_of_very_large_vocabularies(eng):
+    """More slices to a row than ids are sorted by."""
+    check_rules(eng, 9, 600001, seed=7, hist=(3000, 2000), biases=700, masks="rows")
+
+
+def test_rules_rows_without_ids_between(eng):
+    """Rows with many ids, with none and with many again, one after another in the same block."""
+    from turt_b200.runtime import make_logit_rules
+    rows, vocab = 900, 6000
+    rs = np.random.default_rng(8)
+    lens = rs.choice([0, 0, 1, 500, 5000], rows)
+    start = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32).cuda()
+    ids = torch.tensor(rs.integers(0, vocab, int(start[-1])), dtype=torch.int32).cuda()
+    rep = torch.full((rows,), 2.0, device="cuda")
+    x = torch.randn(rows, vocab, device="cuda")
+    y = torch.empty_like(x)
+    eng.logitRules(x.data_ptr(), vocab, y.data_ptr(), vocab, rows, vocab,
+                   make_logit_rules(tokens=ids.data_ptr(), token_start=start.data_ptr(), repetition=rep.data_ptr()))
+    eng.ctx.synchronize()
+    seen = torch.zeros(rows, vocab, dtype=torch.bool)
+    row = np.repeat(np.arange(rows), lens)
+    seen[torch.tensor(row), ids.cpu().long()] = True
+    x = x.cpu()
+    assert torch.equal(y.cpu(), torch.where(seen, torch.where(x > 0, x / 2, x * 2), x))
 
 
 def test_rules_repeated_ids_count(eng):

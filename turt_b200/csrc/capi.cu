@@ -42,6 +42,17 @@ int ctx_check_flags(turt_ctx* ctx) {
   return OK;
 }
 
+int sm_count(int device, int* out) {
+  static std::atomic<int> known[64];
+  int n = known[device & 63].load(std::memory_order_relaxed);
+  if (!n) {
+    TURT_CHECK_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
+    known[device & 63].store(n, std::memory_order_relaxed);
+  }
+  *out = n;
+  return OK;
+}
+
 }  // namespace turt
 
 using namespace turt;

@@ -28,4 +28,6 @@ struct turt_ctx {
 namespace turt {
 // Reads and clears the device flags; returns the matching status.
 int ctx_check_flags(turt_ctx* ctx);
+// Multiprocessors of a device.
+int sm_count(int device, int* out);
 }  // namespace turt

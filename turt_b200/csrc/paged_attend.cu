@@ -1010,17 +1010,6 @@ __global__ void __launch_bounds__(P::WARPS * 32)
   }
 }
 
-int sm_count(int device, int* out) {
-  static std::atomic<int> known[64];
-  int n = known[device & 63].load(std::memory_order_relaxed);
-  if (!n) {
-    TURT_CHECK_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device));
-    known[device & 63].store(n, std::memory_order_relaxed);
-  }
-  *out = n;
-  return OK;
-}
-
 // Tensor map of a paged cache: [page][head][slot][dim], boxes of `rows` slots x `cols` elements.
 int cache_map(CUtensorMap* map, const void* base, int dtype, const PagedLayout& kv, int cols, int rows, bool swizzle) {
   const TensorMapEncode enc = tensor_map_encode();

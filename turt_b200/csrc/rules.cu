@@ -5,17 +5,21 @@
 //   x = logits;  seen: x = x > 0 ? x / rep : x * rep;  n > 0: x -= freq * n, x -= pres;
 //   x += bias[v];  mask bit 0: x = -infinity
 //
-// One pass over the logits: a block owns a slice of one row's vocabulary, counts the row's ids that
-// fall into the slice in shared memory (integer atomics: the counts do not depend on their order)
-// and applies everything while the slice streams through.
+// One pass over the logits, bound by their memory traffic.  A block owns a slice of one row's
+// vocabulary and asks for all of its logits and mask bits at once.  While they arrive it counts the
+// row's ids that fall into the slice in shared memory (integer atomics: the counts do not depend on
+// their order) and lists each touched id once; then a thread per touched id, and not the stream, works
+// out the new logit, which takes the count's place; the stream only picks it up.  Every block of a row
+// reads all of the row's ids, from L2, which is why slices are as long as filling the GPU allows.
 #include "../../include/turt_cuda.h"
+#include <algorithm>
+
 #include "ctx.cuh"
 
 namespace turt {
 namespace {
 
-constexpr int kRuleThreads = 256;
-constexpr uint32_t kSeen = 0x80000000u;  // count word: bit 31 = in the prompt, the rest = times generated
+constexpr uint32_t kSeen = 0x80000000u;  // count word: in the prompt; the other bits = times generated
 constexpr uint32_t kNoMask = 0xFFFFFFFFu;
 
 struct RuleArgs {
@@ -23,127 +27,509 @@ struct RuleArgs {
   const float* in;
   float* out;
   size_t ld, out_ld;
-  int vocab, slice;
+  int vocab;
   int* flags;
 };
 
 struct RowRules {
   float rep, freq, pres;
-  const uint32_t* mask;
 };
 
-__device__ __forceinline__ float apply_rules(const RowRules& w, float x, uint32_t c, float bias, bool open) {
-  if (c) {
-    x = x > 0.f ? x / w.rep : x * w.rep;
-    const uint32_t n = c & ~kSeen;
-    if (n) {
-      x -= w.freq * (float)n;
-      x -= w.pres;
-    }
+__device__ __forceinline__ float penalise(const RowRules& w, float x, uint32_t c) {
+  if (c) x = x > 0.f ? x / w.rep : x * w.rep;
+  const uint32_t n = c & ~kSeen;
+  if (n) {
+    x -= w.freq * (float)n;
+    x -= w.pres;
   }
-  x += bias;
-  return open ? x : -INFINITY;
+  return x;
 }
 
-// Slices are cut where a float4 of the row starts: `lead` elements lie between that boundary and the row's
-// first, so position e of the slice's arrays is id e - lead.  VEC: 16-byte loads and stores.
-template <bool VEC>
-__global__ void __launch_bounds__(kRuleThreads) k_logit_rules(const __grid_constant__ RuleArgs a) {
-  extern __shared__ __align__(16) uint32_t cnt[];  // [slice] counts, [slice] biases
-  float* bias = reinterpret_cast<float*>(cnt + a.slice);
-  const int r = blockIdx.y, V = a.vocab;
+// Slices are cut where a float4 of the row starts: `lead` elements lie between that boundary and the
+// row's first, so position e of the slice is id s0 + e.  VEC: in and out share their boundaries.
+template <int THREADS, int NV, bool VEC>
+__global__ void __launch_bounds__(THREADS, 1536 / THREADS) k_logit_rules(const __grid_constant__ RuleArgs a) {
+  constexpr int SLICE = THREADS * NV * 4;
+  extern __shared__ __align__(16) uint32_t cnt[];  // [SLICE] counts, then new logits
+  uint32_t* touched = cnt + SLICE;                 // a bit per id with a new logit
+  uint16_t* list = reinterpret_cast<uint16_t*>(touched + SLICE / 32);
+  __shared__ uint32_t n_list;
+  const int r = blockIdx.y, V = a.vocab, tid = threadIdx.x;
   const float* in = a.in + (size_t)r * a.ld;
   float* out = a.out + (size_t)r * a.out_ld;
   const int lead = VEC ? (int)((reinterpret_cast<uintptr_t>(in) >> 2) & 3) : 0;
-  const int s0 = blockIdx.x * a.slice - lead;  // id of the slice's first position (may be negative)
-  const bool first = blockIdx.x == 0;
+  const int s0 = blockIdx.x * SLICE - lead;
   if (s0 >= V) return;
+  const bool listed = a.r.tokens != nullptr || a.r.bias_ids != nullptr;
+  if (listed) {
+#pragma unroll
+    for (int k = 0; k < NV; k++) *reinterpret_cast<uint4*>(cnt + (k * THREADS + tid) * 4) = make_uint4(0, 0, 0, 0);
+    for (int e = tid; e < SLICE / 32; e += THREADS) touched[e] = 0;
+    if (tid == 0) n_list = 0;
+  }
   pdl_wait();
   pdl_trigger();
-  const bool hist = a.r.tokens != nullptr, biased = a.r.bias_ids != nullptr;
-  if (hist)
-    for (int e = threadIdx.x * 4; e < a.slice; e += kRuleThreads * 4) *reinterpret_cast<uint4*>(cnt + e) = make_uint4(0, 0, 0, 0);
-  if (biased)
-    for (int e = threadIdx.x * 4; e < a.slice; e += kRuleThreads * 4)
-      *reinterpret_cast<float4*>(bias + e) = make_float4(0.f, 0.f, 0.f, 0.f);
-  __syncthreads();
   bool bad = false;
-  if (hist) {
-    const uint32_t i1 = a.r.token_start[r + 1], g = a.r.generated_start ? a.r.generated_start[r] : 0xFFFFFFFFu;
-    for (uint32_t i = a.r.token_start[r] + threadIdx.x; i < i1; i += kRuleThreads) {
-      const uint32_t id = a.r.tokens[i];
-      const uint32_t e = id - (uint32_t)s0;
-      if (id >= (uint32_t)V)
-        bad = true;
-      else if (e < (uint32_t)a.slice) {
-        if (i >= g)
-          atomicAdd(&cnt[e], 1u);
-        else
-          atomicOr(&cnt[e], kSeen);
-      }
-    }
-  }
-  if (biased) {
-    const uint32_t i0 = a.r.bias_start[r], i1 = a.r.bias_start[r + 1];
-    for (uint32_t i = i0 + threadIdx.x; i < i1; i += kRuleThreads) {
-      const uint32_t id = a.r.bias_ids[i];
-      const uint32_t e = id - (uint32_t)s0;
-      if (id >= (uint32_t)V || (first && i > i0 && a.r.bias_ids[i - 1] >= id))
-        bad = true;
-      else if (e < (uint32_t)a.slice)
-        bias[e] = a.r.bias[i];
-    }
-  }
-  RowRules w;
-  w.rep = a.r.repetition ? a.r.repetition[r] : 1.f;
-  w.freq = a.r.frequency ? a.r.frequency[r] : 0.f;
-  w.pres = a.r.presence ? a.r.presence[r] : 0.f;
-  w.mask = nullptr;
+  const uint32_t* mask = nullptr;
   if (a.r.mask) {
     const uint32_t m = a.r.mask_row ? a.r.mask_row[r] : (uint32_t)r;
     if (m < (uint32_t)a.r.n_masks)
-      w.mask = a.r.mask + (size_t)m * ((V + 31) / 32);
+      mask = a.r.mask + (size_t)m * ((V + 31) / 32);
     else if (m != kNoMask)
       bad = true;
   }
-  if (bad) atomicExch(&a.flags[FLAG_RANGE], RANGE_RULE);
-  __syncthreads();
-  if (VEC) {
-    for (int e = threadIdx.x * 4; e < a.slice; e += kRuleThreads * 4) {
-      const int id = s0 + e;
-      if (id >= V) break;
-      uint4 c = hist ? *reinterpret_cast<uint4*>(cnt + e) : make_uint4(0, 0, 0, 0);
-      float4 bs = biased ? *reinterpret_cast<float4*>(bias + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-      uint32_t open = 0xF;
-      if (w.mask) {
-        open = 0;
+  float4 x[NV];
+  uint32_t open[NV];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (id + j >= 0 && id + j < V) open |= ((w.mask[(id + j) >> 5] >> ((id + j) & 31)) & 1) << j;
-      }
-      if (id >= 0 && id + 4 <= V) {
-        float4 x = *reinterpret_cast<const float4*>(in + id);
-        x.x = apply_rules(w, x.x, c.x, bs.x, open & 1);
-        x.y = apply_rules(w, x.y, c.y, bs.y, open & 2);
-        x.z = apply_rules(w, x.z, c.z, bs.z, open & 4);
-        x.w = apply_rules(w, x.w, c.w, bs.w, open & 8);
-        *reinterpret_cast<float4*>(out + id) = x;
-      } else {
-        const uint32_t cc[4] = {c.x, c.y, c.z, c.w};
-        const float bb[4] = {bs.x, bs.y, bs.z, bs.w};
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (id + j >= 0 && id + j < V) out[id + j] = apply_rules(w, in[id + j], cc[j], bb[j], (open >> j) & 1);
-      }
+  for (int k = 0; k < NV; k++) {
+    const int id = s0 + (k * THREADS + tid) * 4;
+    if (VEC && id >= 0 && id + 4 <= V) {
+      x[k] = *reinterpret_cast<const float4*>(in + id);
+    } else {
+      x[k].x = id >= 0 && id < V ? in[id] : 0.f;
+      x[k].y = id + 1 >= 0 && id + 1 < V ? in[id + 1] : 0.f;
+      x[k].z = id + 2 >= 0 && id + 2 < V ? in[id + 2] : 0.f;
+      x[k].w = id + 3 >= 0 && id + 3 < V ? in[id + 3] : 0.f;
     }
-  } else {
-    for (int e = threadIdx.x; e < a.slice; e += kRuleThreads) {
-      const int id = s0 + e;
-      if (id >= V) break;
-      const bool open = !w.mask || ((w.mask[id >> 5] >> (id & 31)) & 1);
-      out[id] = apply_rules(w, in[id], hist ? cnt[e] : 0, biased ? bias[e] : 0.f, open);
+    open[k] = 0xF;
+    if (mask && id < V) {
+      const int at = max(id, 0), word = at >> 5, words = (V + 31) >> 5;
+      const uint32_t low = mask[word], high = (at & 31) > 28 && word + 1 < words ? mask[word + 1] : 0;
+      open[k] = __funnelshift_r(low, high, at & 31) << (at - id);
     }
   }
+  if (listed) {
+    __syncthreads();
+    if (a.r.tokens) {
+      const uint32_t i0 = a.r.token_start[r], i1 = a.r.token_start[r + 1];
+      const uint32_t g = a.r.generated_start ? a.r.generated_start[r] : 0xFFFFFFFFu;
+      auto count = [&](uint32_t i, uint32_t id) {
+        const uint32_t e = id - (uint32_t)s0;
+        bad |= id >= (uint32_t)V;
+        if (e < (uint32_t)SLICE && id < (uint32_t)V) {
+          const uint32_t old = i >= g ? atomicAdd(&cnt[e], 1u) : atomicOr(&cnt[e], kSeen);
+          if (old == 0) list[atomicAdd(&n_list, 1u)] = (uint16_t)e;
+        }
+      };
+      // four ids at a time where they lie in one 16-byte unit
+      const uint32_t skew = (uint32_t)(reinterpret_cast<uintptr_t>(a.r.tokens) >> 2) & 3;
+      for (uint64_t q = ((uint64_t)i0 + skew) / 4 + tid; q * 4 < (uint64_t)i1 + skew; q += THREADS) {
+        const int64_t i = (int64_t)(q * 4) - skew;
+        if (i >= i0 && i + 4 <= i1) {
+          const uint4 u = *reinterpret_cast<const uint4*>(a.r.tokens + i);
+          count((uint32_t)i, u.x);
+          count((uint32_t)i + 1, u.y);
+          count((uint32_t)i + 2, u.z);
+          count((uint32_t)i + 3, u.w);
+        } else {
+          for (int64_t x = max(i, (int64_t)i0); x < min(i + 4, (int64_t)i1); x++) count((uint32_t)x, a.r.tokens[x]);
+        }
+      }
+    }
+    uint32_t b0 = 0, b1 = 0;
+    if (a.r.bias_ids) {
+      b0 = a.r.bias_start[r];
+      b1 = a.r.bias_start[r + 1];
+      for (uint32_t i = b0 + tid; i < b1; i += THREADS) {
+        const uint32_t id = a.r.bias_ids[i], e = id - (uint32_t)s0;
+        bad |= id >= (uint32_t)V || (blockIdx.x == 0 && i > b0 && a.r.bias_ids[i - 1] >= id);
+        if (e < (uint32_t)SLICE && id < (uint32_t)V) atomicOr(&touched[e >> 5], 1u << (e & 31));
+      }
+    }
+    RowRules w;
+    w.rep = a.r.repetition ? a.r.repetition[r] : 1.f;
+    w.freq = a.r.frequency ? a.r.frequency[r] : 0.f;
+    w.pres = a.r.presence ? a.r.presence[r] : 0.f;
+    __syncthreads();
+    // ids with a bias (their bits are set already) belong to it, the others to the list
+    for (uint32_t i = b0 + tid; i < b1; i += THREADS) {
+      const uint32_t id = a.r.bias_ids[i], e = id - (uint32_t)s0;
+      if (e < (uint32_t)SLICE && id < (uint32_t)V)
+        cnt[e] = __float_as_uint(penalise(w, in[id], cnt[e]) + a.r.bias[i]);
+    }
+    for (uint32_t i = tid; i < n_list; i += THREADS) {
+      const uint32_t e = list[i], bit = 1u << (e & 31);
+      if (!(atomicOr(&touched[e >> 5], bit) & bit))
+        cnt[e] = __float_as_uint(penalise(w, in[(int)e + s0], cnt[e]));
+    }
+    __syncthreads();
+  }
+  if (bad) atomicExch(&a.flags[FLAG_RANGE], RANGE_RULE);
+#pragma unroll
+  for (int k = 0; k < NV; k++) {
+    const int e = (k * THREADS + tid) * 4, id = s0 + e;
+    if (id >= V) break;
+    if (listed) {
+      const uint32_t t = touched[e >> 5] >> (e & 31);
+      if (t & 0xF) {
+        const float4 y = *reinterpret_cast<const float4*>(cnt + e);
+        if (t & 1) x[k].x = y.x;
+        if (t & 2) x[k].y = y.y;
+        if (t & 4) x[k].z = y.z;
+        if (t & 8) x[k].w = y.w;
+      }
+    }
+    if (!(open[k] & 1)) x[k].x = -INFINITY;
+    if (!(open[k] & 2)) x[k].y = -INFINITY;
+    if (!(open[k] & 4)) x[k].z = -INFINITY;
+    if (!(open[k] & 8)) x[k].w = -INFINITY;
+    if (VEC && id >= 0 && id + 4 <= V) {
+      *reinterpret_cast<float4*>(out + id) = x[k];
+    } else {
+      if (id >= 0) out[id] = x[k].x;
+      if (id + 1 >= 0 && id + 1 < V) out[id + 1] = x[k].y;
+      if (id + 2 >= 0 && id + 2 < V) out[id + 2] = x[k].z;
+      if (id + 3 >= 0 && id + 3 < V) out[id + 3] = x[k].w;
+    }
+  }
+}
+
+template <int THREADS, int NV>
+int rules_launch(cudaStream_t st, const RuleArgs& a, int rows, bool vec) {
+  static std::atomic<uint64_t> done{0}, done_vec{0};
+  constexpr int SLICE = THREADS * NV * 4, SMEM = SLICE * 4 + SLICE / 8 + SLICE * 2;
+  const dim3 grid(ceil_div((long)a.vocab + 3, SLICE), rows);
+  if (vec) {
+    RC(smem_attr_per_device(done_vec, k_logit_rules<THREADS, NV, true>, SMEM));
+    TURT_CHECK_CUDA(launch_pdl(k_logit_rules<THREADS, NV, true>, grid, dim3(THREADS), SMEM, st, a));
+  } else {
+    RC(smem_attr_per_device(done, k_logit_rules<THREADS, NV, false>, SMEM));
+    TURT_CHECK_CUDA(launch_pdl(k_logit_rules<THREADS, NV, false>, grid, dim3(THREADS), SMEM, st, a));
+  }
+  TURT_LAUNCH_CHECK();
+  return OK;
+}
+
+// The same rules for large batches, as a pipeline: one block per SM walks over slices of up to
+// kMostIds ids; a producer warp brings the logits, the row's ids, its biases and its mask bits of the
+// slices ahead into a ring of shared memory, sixteen warps work in place on the slice that has
+// arrived and store it.  The blocks of k_logit_rules wait for their ids, then for the touched logits,
+// with nothing else to do; here both lie in shared memory before they are wanted.  When a block comes to
+// a row of several slices it sorts the row's ids by slice once, so that each slice sees only its own.
+constexpr int kMostIds = 8192, kRing = 3, kWorkers = 512;
+constexpr int kTokenRoom = 4096, kBiasRoom = 512;  // per slice; what is beyond is read from L2
+constexpr int kSorted = 64;                        // slices of a row up to which its ids are sorted
+constexpr int kWaitSite = 41;                      // reported when a wait of the pipeline runs out
+
+struct RuleSlice {
+  int row, s0;                // id of the slice's first position (negative: before the row)
+  uint32_t i0, i1, made;      // ids of the row; from `made` on generated
+  uint32_t b0, b1;            // biases
+  uint32_t word0;             // first mask word here
+  int masked;
+  RowRules w;
+};
+
+struct __align__(128) RuleStage {
+  float x[kMostIds];
+  uint32_t tokens[kTokenRoom + 8];
+  uint32_t bias_ids[kBiasRoom + 8];
+  float bias[kBiasRoom + 8];
+  uint32_t mask[kMostIds / 32 + 8];
+  RuleSlice s;
+};
+
+struct RuleShared {
+  RuleStage ring[kRing];
+  uint32_t cnt[kMostIds];  // all zero between slices
+  uint16_t list[kMostIds];
+  uint32_t sorted[kTokenRoom];  // ids by slice, bit 31: generated
+  uint32_t bins[kSorted + 1];   // sizes, then where each slice's ids begin
+  uint64_t full[kRing], empty[kRing];
+  uint32_t n_list[2];  // by turns
+};
+
+// Words between a place and the 16-byte boundary before it.
+__device__ __forceinline__ uint32_t skew_of(const void* p) { return (uint32_t)(reinterpret_cast<uintptr_t>(p) >> 2) & 3; }
+
+// One warp: n words to dst, which lies as far from a 16-byte boundary as src.  Whole 16-byte units go by
+// one bulk copy counted by bar, the words at the ends by hand.
+__device__ __forceinline__ void bring(void* dst, const void* src, uint32_t n, uint64_t* bar, int lane) {
+  uint32_t head = (4 - skew_of(src)) & 3;
+  head = min(head, n);
+  const uint32_t body = (n - head) & ~3u, tail = n - head - body;
+  uint32_t* d = static_cast<uint32_t*>(dst);
+  const uint32_t* s = static_cast<const uint32_t*>(src);
+  if (body && lane == 0) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(body * 4) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(d + head)),
+                 "l"(s + head), "r"(body * 4), "r"(smem_u32(bar))
+                 : "memory");
+  }
+  if (lane < head) d[lane] = s[lane];
+  if (lane >= 4 && lane - 4 < tail) d[head + body + lane - 4] = s[head + body + lane - 4];
+}
+
+__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
+
+template <bool VEC>
+__global__ void __launch_bounds__(kWorkers + 32, 1)
+    k_logit_rules_stream(const __grid_constant__ RuleArgs a, int rows, int slices, int slice, uint32_t slice_mul) {
+  extern __shared__ char smem_raw[];
+  RuleShared& sh = *reinterpret_cast<RuleShared*>(smem_raw + (128 - (smem_u32(smem_raw) & 127)) % 128);
+  const int tid = threadIdx.x, lane = tid & 31, V = a.vocab;
+  const long items = (long)rows * slices;
+  const bool sort = slices > 1 && slices <= kSorted;
+  const long first = items * blockIdx.x / gridDim.x, last = items * (blockIdx.x + 1) / gridDim.x;
+  if (tid < kRing) {
+    mbar_init(&sh.full[tid], 1);
+    mbar_init(&sh.empty[tid], kWorkers / 32);
+  }
+  if (tid < 2) sh.n_list[tid] = 0;
+  for (int e = tid; e < kMostIds; e += kWorkers + 32) sh.cnt[e] = 0;
+  mbar_fence_init();
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+
+  if (tid >= kWorkers) {
+    RuleSlice s;
+    s.row = -1;
+    for (long it = first; it < last; it++) {
+      const int k = (int)(it - first), at = k % kRing;
+      RuleStage& st = sh.ring[at];
+      const int row = (int)(it / slices);
+      const float* in = a.in + (size_t)row * a.ld;
+      const bool fresh = row != s.row;
+      if (fresh) {
+        s.row = row;
+        s.i0 = s.i1 = s.b0 = s.b1 = 0;
+        s.made = 0xFFFFFFFFu;
+        if (a.r.tokens) {
+          s.i0 = a.r.token_start[row];
+          s.i1 = max(s.i0, a.r.token_start[row + 1]);
+          if (a.r.generated_start) s.made = a.r.generated_start[row];
+        }
+        if (a.r.bias_ids) {
+          s.b0 = a.r.bias_start[row];
+          s.b1 = max(s.b0, a.r.bias_start[row + 1]);
+        }
+        s.w.rep = a.r.repetition ? a.r.repetition[row] : 1.f;
+        s.w.freq = a.r.frequency ? a.r.frequency[row] : 0.f;
+        s.w.pres = a.r.presence ? a.r.presence[row] : 0.f;
+        s.masked = -1;
+        if (a.r.mask) {
+          const uint32_t m = a.r.mask_row ? a.r.mask_row[row] : (uint32_t)row;
+          if (m < (uint32_t)a.r.n_masks)
+            s.masked = (int)m;
+          else if (m != kNoMask && lane == 0)
+            atomicExch(&a.flags[FLAG_RANGE], RANGE_RULE);
+        }
+      }
+      s.s0 = (int)(it - (long)row * slices) * slice - (VEC ? (int)skew_of(in) : 0);
+      const int id0 = max(s.s0, 0), id1 = min(s.s0 + slice, V);
+      s.word0 = id0 >> 5;
+      if (k >= kRing) mbar_wait(&sh.empty[at], (k / kRing - 1) & 1, a.flags, kWaitSite);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (id1 > id0) {
+        // with !VEC a slice may begin anywhere: positions keep the distance to a 16-byte boundary
+        bring(st.x + (VEC ? id0 - s.s0 : skew_of(in + id0)), in + id0, id1 - id0, &sh.full[at], lane);
+        if (s.i1 > s.i0 && (fresh || !sort))
+          bring(st.tokens + skew_of(a.r.tokens + s.i0), a.r.tokens + s.i0, min(s.i1 - s.i0, (uint32_t)kTokenRoom),
+                &sh.full[at], lane);
+        if (s.b1 > s.b0) {
+          const uint32_t n = min(s.b1 - s.b0, (uint32_t)kBiasRoom);
+          bring(st.bias_ids + skew_of(a.r.bias_ids + s.b0), a.r.bias_ids + s.b0, n, &sh.full[at], lane);
+          bring(st.bias + skew_of(a.r.bias + s.b0), a.r.bias + s.b0, n, &sh.full[at], lane);
+        }
+        if (s.masked >= 0) {
+          const uint32_t* m = a.r.mask + (size_t)s.masked * ((V + 31) / 32) + s.word0;
+          bring(st.mask + skew_of(m), m, ((id1 - 1) >> 5) - s.word0 + 1, &sh.full[at], lane);
+        }
+      }
+      if (lane == 0) st.s = s;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.full[at]);
+    }
+    return;
+  }
+
+  bool bad = false;
+  int turn = 0;  // slices of rows with ids so far
+  int sorted_row = -1;
+  for (long it = first; it < last; it++) {
+    const int k = (int)(it - first), at = k % kRing;
+    RuleStage& st = sh.ring[at];
+    mbar_wait(&sh.full[at], (k / kRing) & 1, a.flags, kWaitSite);
+    const RuleSlice& s = st.s;
+    const int s0 = s.s0, id0 = max(s0, 0), id1 = min(s0 + slice, V);
+    if (id1 > id0) {
+      float* x = st.x + (VEC ? 0 : (int)skew_of(a.in + (size_t)s.row * a.ld + id0));  // position e = id - s0
+      const uint32_t n_tok = s.i1 - s.i0, n_bias = s.b1 - s.b0, span = id1 - id0;
+      if (n_tok) {
+        const uint32_t skew = skew_of(a.r.tokens + s.i0), here = min(n_tok, (uint32_t)kTokenRoom);
+        const uint32_t made = s.made > s.i0 ? s.made - s.i0 : 0;
+        uint32_t most = 0;
+        auto count = [&](bool gen, uint32_t id) {
+          most = max(most, id);
+          if (id - (uint32_t)id0 < span) {
+            const uint32_t p = id - (uint32_t)s0;
+            uint32_t old;
+            if (gen)
+              old = atomicAdd(&sh.cnt[p], 1u);
+            else
+              old = atomicOr(&sh.cnt[p], kSeen);
+            if (old == 0) sh.list[atomicAdd(&sh.n_list[turn & 1], 1u)] = (uint16_t)p;
+          }
+        };
+        if (sort) {
+          const int bin = (int)(it - (long)s.row * slices);
+          if (s.row != sorted_row) {
+            sorted_row = s.row;
+            const uint32_t lead = (uint32_t)(bin * slice - s0);
+            constexpr int PER = kTokenRoom / kWorkers;
+            uint32_t mine[PER], rank[PER];
+            if (tid <= kSorted) sh.bins[tid] = 0;
+            workers_sync();
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+              const uint32_t i = j * kWorkers + tid;
+              if (j * kWorkers >= here) break;
+              const uint32_t id = i < here ? st.tokens[skew + i] : 0xFFFFFFFFu;
+              if (i < here) most = max(most, id);
+              const uint32_t to = id < (uint32_t)V ? __umulhi(id + lead, slice_mul) : kSorted;
+              const uint32_t same = __match_any_sync(0xffffffffu, to);
+              const int leader = __ffs(same) - 1;
+              uint32_t base = 0;
+              if (lane == leader && to < kSorted) base = atomicAdd(&sh.bins[to], (uint32_t)__popc(same));
+              rank[j] = __shfl_sync(0xffffffffu, base, leader) + __popc(same & ((1u << lane) - 1));
+              mine[j] = to < kSorted ? id | (i >= made ? kSeen : 0) : 0xFFFFFFFFu;
+            }
+            workers_sync();
+            if (tid < 32) {  // where each slice's ids begin
+              const uint32_t c0 = sh.bins[2 * lane], c1 = sh.bins[2 * lane + 1];
+              uint32_t sum = c0 + c1;
+#pragma unroll
+              for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+              }
+              sh.bins[2 * lane] = sum - c0 - c1;
+              sh.bins[2 * lane + 1] = sum - c1;
+              if (lane == 31) sh.bins[kSorted] = sum;
+            }
+            workers_sync();
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+              if (j * kWorkers >= here) break;
+              if (mine[j] != 0xFFFFFFFFu) sh.sorted[sh.bins[__umulhi((mine[j] & ~kSeen) + lead, slice_mul)] + rank[j]] = mine[j];
+            }
+            workers_sync();
+          }
+          for (uint32_t i = sh.bins[bin] + tid; i < sh.bins[bin + 1]; i += kWorkers)
+            count((sh.sorted[i] & kSeen) != 0, sh.sorted[i] & ~kSeen);
+        } else {
+          for (uint32_t q = tid * 4; q < here + skew; q += kWorkers * 4) {  // ids q - skew .. + 3
+            const uint4 u = *reinterpret_cast<const uint4*>(st.tokens + q);
+            if (q >= skew && q + 4 <= here + skew) {
+              count(q - skew >= made, u.x);
+              count(q + 1 - skew >= made, u.y);
+              count(q + 2 - skew >= made, u.z);
+              count(q + 3 - skew >= made, u.w);
+            } else {
+              if (q >= skew) count(q - skew >= made, u.x);
+              if (q + 1 >= skew && q + 1 < here + skew) count(q + 1 - skew >= made, u.y);
+              if (q + 2 >= skew && q + 2 < here + skew) count(q + 2 - skew >= made, u.z);
+              if (q + 3 >= skew && q + 3 < here + skew) count(q + 3 - skew >= made, u.w);
+            }
+          }
+        }
+        for (uint32_t i = here + tid; i < n_tok; i += kWorkers) count(i >= made, a.r.tokens[s.i0 + i]);
+        bad |= most >= (uint32_t)V;
+        workers_sync();
+        const uint32_t n = sh.n_list[turn & 1];
+        for (uint32_t i = tid; i < n; i += kWorkers) {
+          const uint32_t p = sh.list[i];
+          x[p] = penalise(s.w, x[p], sh.cnt[p]);
+          sh.cnt[p] = 0;
+        }
+        turn++;
+        if (tid == 0) sh.n_list[turn & 1] = 0;
+        workers_sync();
+      }
+      if (n_bias) {
+        const uint32_t* ids = st.bias_ids + skew_of(a.r.bias_ids + s.b0);
+        const float* val = st.bias + skew_of(a.r.bias + s.b0);
+        const uint32_t here = min(n_bias, (uint32_t)kBiasRoom);
+        for (uint32_t i = tid; i < n_bias; i += kWorkers) {
+          const uint32_t id = i < here ? ids[i] : a.r.bias_ids[s.b0 + i];
+          bad |= id >= (uint32_t)V || (s0 <= 0 && i > 0 && (i <= here ? ids[i - 1] : a.r.bias_ids[s.b0 + i - 1]) >= id);
+          if (id - (uint32_t)id0 < span) x[id - s0] += i < here ? val[i] : a.r.bias[s.b0 + i];
+        }
+        workers_sync();
+      }
+      const bool masked = s.masked >= 0;
+      const uint32_t* mask =
+          masked ? st.mask + skew_of(a.r.mask + (size_t)s.masked * ((V + 31) / 32) + s.word0) : nullptr;
+      const uint32_t words = ((id1 - 1) >> 5) - s.word0 + 1;
+      float* out = a.out + (size_t)s.row * a.out_ld;
+      if (VEC) {
+        for (int e = tid * 4; e < slice; e += kWorkers * 4) {
+          const int id = s0 + e;
+          if (id >= id1) break;
+          float4 y = *reinterpret_cast<const float4*>(x + e);
+          if (masked) {
+            const int from = max(id, 0);
+            const uint32_t wd = (from >> 5) - s.word0, low = mask[wd], high = wd + 1 < words ? mask[wd + 1] : 0;
+            const uint32_t open = __funnelshift_r(low, high, from & 31) << (from - id);
+            if (!(open & 1)) y.x = -INFINITY;
+            if (!(open & 2)) y.y = -INFINITY;
+            if (!(open & 4)) y.z = -INFINITY;
+            if (!(open & 8)) y.w = -INFINITY;
+          }
+          if (id >= 0 && id + 4 <= id1) {
+            *reinterpret_cast<float4*>(out + id) = y;
+          } else {
+            if (id >= 0) out[id] = y.x;
+            if (id + 1 >= 0 && id + 1 < id1) out[id + 1] = y.y;
+            if (id + 2 >= 0 && id + 2 < id1) out[id + 2] = y.z;
+            if (id + 3 >= 0 && id + 3 < id1) out[id + 3] = y.w;
+          }
+        }
+      } else {
+        for (int id = id0 + tid; id < id1; id += kWorkers) {
+          float y = x[id - s0];
+          if (masked && !((mask[(id >> 5) - s.word0] >> (id & 31)) & 1)) y = -INFINITY;
+          out[id] = y;
+        }
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // in order before the next copies into this stage
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.empty[at]);
+  }
+  if (bad) atomicExch(&a.flags[FLAG_RANGE], RANGE_RULE);
+}
+
+// How a row is cut: the number of slices (of kMostIds at most) that gives the fullest last turn.
+int rules_stream(turt_ctx* ctx, const RuleArgs& a, int rows, bool vec) {
+  static std::atomic<uint64_t> done{0}, done_vec{0};
+  int sms = 0;
+  RC(sm_count(ctx->device, &sms));
+  const int extra = vec ? 3 : 0, least = ceil_div((long)a.vocab + extra, kMostIds - 4);
+  int slices = least, slice = 0;
+  long best = 0;
+  for (int n = least; n <= 2 * least + 2; n++) {
+    const int len = (ceil_div((long)a.vocab + extra, n) + 3) & ~3;
+    const long cost = (long)ceil_div((long)rows * n, sms) * (len + 512);  // 512: what a slice costs besides its ids
+    if (slice == 0 || cost < best) {
+      best = cost;
+      slices = n;
+      slice = len;
+    }
+  }
+  slices = ceil_div((long)a.vocab + extra, slice);
+  static_assert(sizeof(RuleShared) + 128 <= 227 * 1024, "shared memory");
+  const int smem = (int)sizeof(RuleShared) + 128, grid = (int)std::min((long)rows * slices, (long)sms);
+  auto kern = vec ? k_logit_rules_stream<true> : k_logit_rules_stream<false>;
+  RC(smem_attr_per_device(vec ? done_vec : done, kern, smem));
+  TURT_CHECK_CUDA(launch_pdl(kern, dim3(grid), dim3(kWorkers + 32), smem, ctx->stream, a, rows, slices, slice,
+                             (uint32_t)(((1ull << 32) + slice - 1) / slice)));
+  TURT_LAUNCH_CHECK();
+  return OK;
 }
 
 }  // namespace
@@ -176,12 +562,10 @@ extern "C" int turt_logit_rules_apply(turt_ctx* ctx, const float* logits, size_t
   a.ld = ld, a.out_ld = out_ld;
   a.vocab = vocab;
   a.flags = ctx->flags;
-  a.slice = 4096;
   // every row of in and out starts equally far from a 16-byte boundary
   const bool vec = ((uintptr_t)logits & 15) == ((uintptr_t)out & 15) && (rows == 1 || ld % 4 == out_ld % 4);
-  const size_t smem = (size_t)a.slice * 8;
-  const dim3 grid(ceil_div((long)vocab + 3, a.slice), rows);
-  TURT_CHECK_CUDA(launch_pdl(vec ? k_logit_rules<true> : k_logit_rules<false>, grid, dim3(kRuleThreads), smem, ctx->stream, a));
-  TURT_LAUNCH_CHECK();
-  return OK;
+  const long enough = 4 * 148;
+  if (rows * (long)ceil_div(vocab, kMostIds) >= enough) return rules_stream(ctx, a, rows, vec);
+  if (rows * (long)ceil_div(vocab, 4096) >= enough) return rules_launch<256, 4>(ctx->stream, a, rows, vec);
+  return rules_launch<128, 2>(ctx->stream, a, rows, vec);
 }
