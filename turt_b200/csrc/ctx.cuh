@@ -19,10 +19,6 @@ struct turt_ctx {
   std::map<std::tuple<int, int, float>, float2*> rope_tables;
   void* scratch = nullptr;  // grow-only device scratch of the standalone fused kernels
   size_t scratch_bytes = 0;
-  // Rotation frequencies of the last turt_paged_append, by (rot_dim, base).
-  double rot_freq[128] = {};
-  int rot_dim = 0;
-  float rot_base = 0.0f;
 };
 
 namespace turt {

@@ -68,7 +68,9 @@ namespace {
 //   a = position * base^(-2m / rot)
 // A position of 10^5 and more leaves an fp32 product a with an error of whole hundredths of a
 // turn, so a / pi is formed and reduced to [-1, 1] in double and only then rounded for sincospif
-// (error <= 2^-25 half turns).  The frequencies come from the host as kernel parameters.
+// (error <= 2^-25 half turns).  Bound by the memory traffic where rows are many and by the chain
+// start -> page table -> store where they are few: a thread asks for its elements before it knows
+// where they go, and a warp looks up one row, 32 entries of `start` at a time.
 struct AppendArgs {
   PagedLayout kv;
   const float *k, *v, *q;
@@ -77,133 +79,189 @@ struct AppendArgs {
   const uint32_t* start;
   size_t ks, vs, qs, qos;
   int heads, rows, rot;
+  int per_block;       // rows per block
+  uint32_t items;      // pieces of VEC elements per row
+  uint64_t row_mul;    // e / items = e * row_mul >> 32 (several rows per block: e < 2^13)
+  uint64_t head_mul;   // e / (dim / VEC) likewise (e < 2^25)
+  double step;         // 2 log2(base) / rot
   int* flags;
-  double freq[128];  // base^(-2m / rot) / pi
 };
 
-// Sequence and position of row i; -1: none.  Raises the range flag where the page table does not
-// hold the position.  Returns the element offset of the position for kv head 0.
-__device__ bool append_slot(const AppendArgs& a, int i, int* pos, size_t* off) {
+constexpr int kAppendThreads = 256, kAppendRows = 8;
+
+// One warp: sequence and position of row i; false where it has none.  Raises the range flag where the
+// page table does not hold the position.  off: the element offset of the position for kv head 0.
+__device__ bool append_slot(const AppendArgs& a, int i, int lane, int* pos, size_t* off) {
   const PagedLayout& kv = a.kv;
   int b = i;
   long long p;
   if (a.start) {
-    if ((uint32_t)i < a.start[0] || (uint32_t)i >= a.start[kv.batch]) return false;
-    int lo = 0, hi = kv.batch - 1;  // the last sequence with start[b] <= i
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.start[mid] <= (uint32_t)i)
-        lo = mid;
-      else
-        hi = mid - 1;
+    // the last sequence with start[b] <= i, in steps of a 32nd of what is left
+    int lo = 0, n = kv.batch;  // it is among lo .. lo + n - 1, or there is none
+    while (n > 1) {
+      const int piece = (n + 31) / 32, x = lo + lane * piece;
+      const uint32_t in = __ballot_sync(0xffffffffu, x < lo + n && a.start[x] <= (uint32_t)i);
+      if (in == 0) return false;
+      const int to = lo + (31 - __clz(in)) * piece;
+      n = min(piece, lo + n - to);
+      lo = to;
     }
     b = lo;
-    if ((uint32_t)i >= a.start[b + 1]) return false;
-    p = (long long)kv.lens[b] - a.start[b + 1] + i;
+    const uint32_t first = a.start[b], next = a.start[b + 1];
+    if ((uint32_t)i < first || (uint32_t)i >= next) return false;
+    p = (long long)kv.lens[b] - next + i;
   } else {
     if (kv.lens[b] == 0) return false;
     p = (long long)kv.lens[b] - 1;
   }
-  const long long page = p / kv.page_size;
   uint32_t id = 0xFFFFFFFFu;
+  const uint32_t page = (uint32_t)p / kv.page_size;
   if (p >= 0 && page < kv.max_pages) id = kv.table[(size_t)b * kv.max_pages + page];
   if (id >= kv.n_pages) {
-    atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
+    if (lane == 0) atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
     return false;
   }
   *pos = (int)p;
-  *off = (size_t)id * kv.page_stride + (size_t)(p - page * kv.page_size) * kv.slot_stride;
+  *off = (size_t)id * kv.page_stride + (size_t)((uint32_t)p - page * kv.page_size) * kv.slot_stride;
   return true;
 }
 
-// One block per row; VEC elements of one head per thread and step.
+template <int VEC>
+struct AppendPiece {
+  const float* src;
+  int r, h, d;  // row of the block, head (queries, keys, values), first element
+  float x[VEC];
+};
+
+template <int VEC>
+__device__ __forceinline__ void append_load(const AppendArgs& a, uint32_t e, int row0, AppendPiece<VEC>& p) {
+  const int heads = a.q ? a.heads : 0, kvh = a.kv.kv_heads, dim = a.kv.dim;
+  p.r = a.per_block > 1 ? (int)(e * a.row_mul >> 32) : 0;
+  const uint32_t in = e - p.r * a.items;
+  p.h = (int)(in * a.head_mul >> 32);
+  p.d = (int)(in - p.h * (dim / VEC)) * VEC;
+  const size_t i = row0 + p.r;
+  if (p.h < heads)
+    p.src = a.q + i * a.qs + (size_t)p.h * dim;
+  else if (p.h < heads + kvh)
+    p.src = a.k + i * a.ks + (size_t)(p.h - heads) * dim;
+  else
+    p.src = a.v + i * a.vs + (size_t)(p.h - heads - kvh) * dim;
+  p.src += p.d;
+  if constexpr (VEC == 8) {
+    *reinterpret_cast<float4*>(p.x) = *reinterpret_cast<const float4*>(p.src);
+    *reinterpret_cast<float4*>(p.x + 4) = *reinterpret_cast<const float4*>(p.src + 4);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) p.x[j] = p.src[j];
+  }
+}
+
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) k_paged_append(const __grid_constant__ AppendArgs a) {
-  __shared__ float2 cs[128];
-  __shared__ size_t s_off;
-  __shared__ int s_pos, s_live;
-  const int i = blockIdx.x;
+__device__ __forceinline__ void append_store(const AppendArgs& a, int row0, const float2* cs, size_t off, AppendPiece<VEC>& p) {
+  const int heads = a.q ? a.heads : 0, kvh = a.kv.kv_heads;
+  if (p.h < heads + kvh) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      if (p.d + j < a.rot) {
+        const float2 r = cs[(p.d + j) >> 1];
+        const float y0 = p.x[j] * r.x - p.x[j + 1] * r.y, y1 = p.x[j] * r.y + p.x[j + 1] * r.x;
+        p.x[j] = y0;
+        p.x[j + 1] = y1;
+      }
+    }
+  }
+  if (p.h < heads) {
+    float* to = a.q_out + (size_t)(row0 + p.r) * a.qos + (size_t)p.h * a.kv.dim + p.d;
+    if constexpr (VEC == 8) {
+      *reinterpret_cast<float4*>(to) = *reinterpret_cast<float4*>(p.x);
+      *reinterpret_cast<float4*>(to + 4) = *reinterpret_cast<float4*>(p.x + 4);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; j++) to[j] = p.x[j];
+    }
+    return;
+  }
+  const bool key = p.h < heads + kvh;
+  T* to = (T*)(key ? a.kc : a.vc) + off + (size_t)(p.h - heads - (key ? 0 : kvh)) * a.kv.head_stride + p.d;
+  alignas(16) T y[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; j++) y[j] = from_f32<T>(p.x[j]);
+  if constexpr (VEC == 8) {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(y) / 16; j++) reinterpret_cast<float4*>(to)[j] = reinterpret_cast<float4*>(y)[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) to[j] = y[j];
+  }
+}
+
+// per_block rows per block; VEC elements of one head per thread and piece, up to four pieces under way.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kAppendThreads) k_paged_append(const __grid_constant__ AppendArgs a) {
+  __shared__ float2 cs[kAppendRows][128];
+  __shared__ size_t s_off[kAppendRows];
+  __shared__ int s_pos[kAppendRows];  // -1: the row goes nowhere
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int row0 = blockIdx.x * a.per_block, n = min(a.per_block, a.rows - row0);
+  const int half = a.rot >> 1;
+  double freq = 0.0;  // base^(-2m / rot) / pi of pair m = tid % half
+  const int m = half ? tid % half : 0;
+  if (half) freq = exp2(-a.step * m) * 0.31830988618379067;
   pdl_wait();
   pdl_trigger();
-  if (threadIdx.x == 0) {
-    int pos = 0;
+  constexpr int AHEAD = 4;
+  AppendPiece<VEC> p[AHEAD];
+  const uint32_t total = n * a.items;
+#pragma unroll
+  for (int k = 0; k < AHEAD; k++)
+    if (tid + k * kAppendThreads < total) append_load<VEC>(a, tid + k * kAppendThreads, row0, p[k]);
+  if (w < n) {
+    int pos = -1;
     size_t off = 0;
-    s_live = append_slot(a, i, &pos, &off);
-    s_pos = pos;
-    s_off = off;
+    if (!append_slot(a, row0 + w, lane, &pos, &off)) pos = -1;
+    if (lane == 0) {
+      s_pos[w] = pos;
+      s_off[w] = off;
+    }
   }
   __syncthreads();
-  if (!s_live) return;
-  for (int m = threadIdx.x; m < a.rot / 2; m += blockDim.x) {
-    const double t = s_pos * a.freq[m];
-    float sn, cn;
-    sincospif((float)(t - 2.0 * rint(0.5 * t)), &sn, &cn);
-    cs[m] = make_float2(cn, sn);
+  if (half) {
+    // a thread keeps its pair and goes through the rows
+    const int lanes = kAppendThreads / half, r0 = tid / half;
+    if (r0 < lanes)
+      for (int r = r0; r < n; r += lanes) {
+        const double t = s_pos[r] * freq;
+        float sn, cn;
+        sincospif((float)(t - 2.0 * rint(0.5 * t)), &sn, &cn);
+        cs[r][m] = make_float2(cn, sn);
+      }
+    __syncthreads();
   }
-  __syncthreads();
-  const int per = a.kv.dim / VEC, heads = a.q ? a.heads : 0, kvh = a.kv.kv_heads;
-  for (int e = threadIdx.x; e < (heads + 2 * kvh) * per; e += blockDim.x) {
-    const int h = e / per, d = (e - h * per) * VEC;
-    const float* src;
-    float* qd = nullptr;
-    T* cd = nullptr;
-    bool turn = true;
-    if (h < heads) {
-      src = a.q + (size_t)i * a.qs + (size_t)h * a.kv.dim + d;
-      qd = a.q_out + (size_t)i * a.qos + (size_t)h * a.kv.dim + d;
-    } else if (h < heads + kvh) {
-      src = a.k + (size_t)i * a.ks + (size_t)(h - heads) * a.kv.dim + d;
-      cd = (T*)a.kc + s_off + (size_t)(h - heads) * a.kv.head_stride + d;
-    } else {
-      src = a.v + (size_t)i * a.vs + (size_t)(h - heads - kvh) * a.kv.dim + d;
-      cd = (T*)a.vc + s_off + (size_t)(h - heads - kvh) * a.kv.head_stride + d;
-      turn = false;
-    }
-    float x[VEC];
-    if constexpr (VEC == 8) {
-      *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
-      *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(src + 4);
-    } else {
+  for (uint32_t e = tid; e < total; e += AHEAD * kAppendThreads) {
 #pragma unroll
-      for (int j = 0; j < VEC; j++) x[j] = src[j];
-    }
-    if (turn) {
+    for (int k = 0; k < AHEAD; k++)
+      if (e + k * kAppendThreads < total && s_pos[p[k].r] >= 0)
+        append_store<T, VEC>(a, row0, cs[p[k].r], s_off[p[k].r], p[k]);
 #pragma unroll
-      for (int j = 0; j < VEC; j += 2) {
-        if (d + j < a.rot) {
-          const float2 r = cs[(d + j) >> 1];
-          const float y0 = x[j] * r.x - x[j + 1] * r.y, y1 = x[j] * r.y + x[j + 1] * r.x;
-          x[j] = y0;
-          x[j + 1] = y1;
-        }
-      }
-    }
-    if (qd) {
-      if constexpr (VEC == 8) {
-        *reinterpret_cast<float4*>(qd) = *reinterpret_cast<float4*>(x);
-        *reinterpret_cast<float4*>(qd + 4) = *reinterpret_cast<float4*>(x + 4);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; j++) qd[j] = x[j];
-      }
-    } else {
-      alignas(16) T y[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; j++) y[j] = from_f32<T>(x[j]);
-      if constexpr (VEC == 8) {
-#pragma unroll
-        for (int j = 0; j < (int)sizeof(y) / 16; j++) reinterpret_cast<float4*>(cd)[j] = reinterpret_cast<float4*>(y)[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; j++) cd[j] = y[j];
-      }
+    for (int k = 0; k < AHEAD; k++) {
+      const uint32_t next = e + (AHEAD + k) * kAppendThreads;
+      if (next < total) append_load<VEC>(a, next, row0, p[k]);
     }
   }
 }
 
-template <typename T>
-int append_launch(cudaStream_t st, const AppendArgs& a, bool vec) {
-  TURT_CHECK_CUDA(launch_pdl(vec ? k_paged_append<T, 8> : k_paged_append<T, 2>, dim3(a.rows), dim3(256), 0, st, a));
+template <typename T, int VEC>
+int append_launch(cudaStream_t st, AppendArgs a) {
+  a.items = (uint32_t)(((a.q ? a.heads : 0) + 2 * a.kv.kv_heads) * (a.kv.dim / VEC));
+  // about four pieces per thread, as long as the blocks fill the GPU twice
+  int per = 1;
+  while (per < kAppendRows && 2 * per * a.items <= 4 * kAppendThreads && a.rows / (2 * per) >= 2 * 148) per *= 2;
+  a.per_block = per;
+  auto mul = [](uint32_t d) { return ((1ull << 32) + d - 1) / d; };
+  a.row_mul = mul(a.items);
+  a.head_mul = mul(a.kv.dim / VEC);
+  TURT_CHECK_CUDA(launch_pdl(k_paged_append<T, VEC>, dim3(ceil_div(a.rows, per)), dim3(kAppendThreads), 0, st, a));
   TURT_LAUNCH_CHECK();
   return OK;
 }
@@ -244,19 +302,15 @@ extern "C" int turt_paged_append(turt_ctx* ctx, const turt_paged_kv* kv, const f
   a.ks = k_stride, a.vs = v_stride, a.qs = q_stride, a.qos = q_out_stride;
   a.heads = n_head, a.rows = rows, a.rot = rot_dim;
   a.flags = ctx->flags;
-  if (rot_dim && (ctx->rot_dim != rot_dim || ctx->rot_base != base)) {
-    for (int m = 0; m < rot_dim / 2; m++) ctx->rot_freq[m] = pow((double)base, -2.0 * m / rot_dim) / M_PI;
-    ctx->rot_dim = rot_dim;
-    ctx->rot_base = base;
-  }
-  for (int m = 0; m < rot_dim / 2; m++) a.freq[m] = ctx->rot_freq[m];
+  a.step = rot_dim ? 2.0 * log2((double)base) / rot_dim : 0.0;
   // 16-byte loads and stores: eight elements of a head per thread
   const size_t per = 16 / cache_type_size(kv->dtype);
   const bool vec = kv->head_dim % 8 == 0 && aligned16(k) && aligned16(v) && k_stride % 4 == 0 && v_stride % 4 == 0 &&
                    (!q || (aligned16(q) && aligned16(q_out) && q_stride % 4 == 0 && q_out_stride % 4 == 0)) &&
                    aligned16(kv->k) && aligned16(kv->v) && a.kv.page_stride % per == 0 && a.kv.head_stride % per == 0 &&
                    a.kv.slot_stride % per == 0;
-  if (kv->dtype == TURT_CACHE_F32) return append_launch<float>(ctx->stream, a, vec);
-  if (kv->dtype == TURT_CACHE_F16) return append_launch<__half>(ctx->stream, a, vec);
-  return append_launch<__nv_bfloat16>(ctx->stream, a, vec);
+  if (kv->dtype == TURT_CACHE_F32) return vec ? append_launch<float, 8>(ctx->stream, a) : append_launch<float, 2>(ctx->stream, a);
+  if (kv->dtype == TURT_CACHE_F16)
+    return vec ? append_launch<__half, 8>(ctx->stream, a) : append_launch<__half, 2>(ctx->stream, a);
+  return vec ? append_launch<__nv_bfloat16, 8>(ctx->stream, a) : append_launch<__nv_bfloat16, 2>(ctx->stream, a);
 }
