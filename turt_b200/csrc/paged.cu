@@ -196,9 +196,11 @@ __device__ __forceinline__ void append_store(const AppendArgs& a, int row0, cons
   }
 }
 
-// per_block rows per block; VEC elements of one head per thread and piece, up to four pieces under way.
+// per_block rows per block; VEC elements of one head per thread and piece.  Resident threads count for
+// more than pieces under way per thread: eight blocks per SM with one piece each measured 47.5 us for
+// 6318 rows of 48 heads of 128 (285 MB), four blocks with four pieces 55 us.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kAppendThreads) k_paged_append(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 8) k_paged_append(const __grid_constant__ AppendArgs a) {
   __shared__ float2 cs[kAppendRows][128];
   __shared__ size_t s_off[kAppendRows];
   __shared__ int s_pos[kAppendRows];  // -1: the row goes nowhere
@@ -210,12 +212,9 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const __grid_co
   if (half) freq = exp2(-a.step * m) * 0.31830988618379067;
   pdl_wait();
   pdl_trigger();
-  constexpr int AHEAD = 4;
-  AppendPiece<VEC> p[AHEAD];
+  AppendPiece<VEC> p;
   const uint32_t total = n * a.items;
-#pragma unroll
-  for (int k = 0; k < AHEAD; k++)
-    if (tid + k * kAppendThreads < total) append_load<VEC>(a, tid + k * kAppendThreads, row0, p[k]);
+  if (tid < total) append_load<VEC>(a, tid, row0, p);
   if (w < n) {
     int pos = -1;
     size_t off = 0;
@@ -238,25 +237,19 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const __grid_co
       }
     __syncthreads();
   }
-  for (uint32_t e = tid; e < total; e += AHEAD * kAppendThreads) {
-#pragma unroll
-    for (int k = 0; k < AHEAD; k++)
-      if (e + k * kAppendThreads < total && s_pos[p[k].r] >= 0)
-        append_store<T, VEC>(a, row0, cs[p[k].r], s_off[p[k].r], p[k]);
-#pragma unroll
-    for (int k = 0; k < AHEAD; k++) {
-      const uint32_t next = e + (AHEAD + k) * kAppendThreads;
-      if (next < total) append_load<VEC>(a, next, row0, p[k]);
-    }
+  for (uint32_t e = tid; e < total; e += kAppendThreads) {
+    if (s_pos[p.r] >= 0) append_store<T, VEC>(a, row0, cs[p.r], s_off[p.r], p);
+    if (e + kAppendThreads < total) append_load<VEC>(a, e + kAppendThreads, row0, p);
   }
 }
 
 template <typename T, int VEC>
 int append_launch(cudaStream_t st, AppendArgs a) {
   a.items = (uint32_t)(((a.q ? a.heads : 0) + 2 * a.kv.kv_heads) * (a.kv.dim / VEC));
-  // about four pieces per thread, as long as the blocks fill the GPU twice
+  // up to six pieces per thread, as long as there are two blocks per SM: 4543 rows of 25 heads of 80
+  // took 18.1 us one to a block, 14.8 two, 14.3 four, 16.4 eight
   int per = 1;
-  while (per < kAppendRows && 2 * per * a.items <= 4 * kAppendThreads && a.rows / (2 * per) >= 2 * 148) per *= 2;
+  while (per < kAppendRows && 2 * per * a.items <= 6 * kAppendThreads && a.rows / (2 * per) >= 2 * 148) per *= 2;
   a.per_block = per;
   auto mul = [](uint32_t d) { return ((1ull << 32) + d - 1) / d; };
   a.row_mul = mul(a.items);

@@ -26,6 +26,7 @@ namespace {
 constexpr int kMaxBlocks = 512;           // counters and partial results in the workspace
 constexpr int kPrefix = 1024;             // entries of the tile prefix held in shared memory
 constexpr int kGroup = 8;                 // heads of a group that a warp treats at once, at most
+constexpr int kPartCost = 1;                // what a sequence part costs besides its tiles, in tiles
 constexpr float kLazy = 8.0f;             // the running max moves when it is this far behind (log2)
 constexpr int kWaitSite = 40;             // reported when a copy's wait runs out
 
@@ -101,14 +102,18 @@ __device__ __forceinline__ Seq seq_of(const AttendArgs& a, int b) {
   return s;
 }
 
-// A place on the line of tiles (sequence, part of a head group, tile).
+// A place on the line: sequence, part of a head group, tile.  On the line a sequence part takes up
+// kPartCost places and then one per tile, so that a warp with many short parts gets fewer tiles.
 template <int KT>
 struct Walk {
   Seq s;
   int b, hc;
   uint32_t t;
+  unsigned long long pos;
   __device__ void next(const AttendArgs& a, int hcs) {
+    pos++;
     if (++t < s.t1) return;
+    pos += kPartCost;
     t = s.t0;
     if (++hc < hcs) return;
     hc = 0;
@@ -661,7 +666,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
   __shared__ unsigned long long pre[kPrefix];
   __shared__ unsigned long long warp_tot[WARPS];
   __shared__ uint32_t warp_long[WARPS], warp_live[WARPS];
-  __shared__ long long seg_id[WARPS * 2];  // first tile (on the line) of the sequence part in each record, -1: none
+  __shared__ long long seg_id[WARPS * 2];  // where on the line the sequence part of each record begins, -1: none
   __shared__ int seg_b[WARPS * 2], seg_hc[WARPS * 2], seg_tiles[WARPS * 2];
   __shared__ int open_first[2], open_parts[2], open_rec[2];  // parts that other blocks share: first block, blocks, record
   __shared__ unsigned s_old[2];
@@ -685,7 +690,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
   pdl_wait();
   pdl_trigger();
 
-  // Tiles before every `step`-th sequence, the longest part, and how many parts there are.
+  // Places before every `step`-th sequence, the longest part, and how many parts there are.
   const int step = (a.kv.batch + kPrefix - 1) / kPrefix, n_pre = step == 1 ? a.kv.batch : (a.kv.batch + step - 1) / step;
   unsigned long long total = 0;
   uint32_t longest = 0, live_seqs = 0;
@@ -697,7 +702,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
       for (int b = e * step; b < min(a.kv.batch, (e + 1) * step); b++) {
         const Seq s = seq_of<KT>(a, b);
         if (s.n == 0 && a.kv.lens[b] != 0 && blockIdx.x == 0) atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
-        sum += s.t1 - s.t0;
+        sum += s.n ? s.t1 - s.t0 + kPartCost : 0;
         most = max(most, s.t1 - s.t0);
         live += s.n != 0;
       }
@@ -739,7 +744,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
     }
   if (total == 0) return;
 
-  // The place of tile u on the line, and the first tile of its sequence part.
+  // The first tile at place u of the line or behind it, and where its sequence part begins.
   auto locate = [&](unsigned long long u, Walk<KT>& at) -> unsigned long long {
     int l = 0, r = n_pre - 1;
     while (l < r) {
@@ -750,16 +755,19 @@ __global__ void __launch_bounds__(P::WARPS * 32)
         r = mid - 1;
     }
     unsigned long long x = pre[l];
+    auto places = [&]() { return at.s.n ? (unsigned long long)(at.s.t1 - at.s.t0 + kPartCost) * hcs : 0; };
     at.b = l * step;
     at.s = seq_of<KT>(a, at.b);
-    while (x + (unsigned long long)(at.s.t1 - at.s.t0) * hcs <= u && at.b + 1 < a.kv.batch) {
-      x += (unsigned long long)(at.s.t1 - at.s.t0) * hcs;
+    while (x + places() <= u && at.b + 1 < a.kv.batch) {
+      x += places();
       at.s = seq_of<KT>(a, ++at.b);
     }
-    const uint32_t in = (uint32_t)(u - x), tiles = at.s.t1 - at.s.t0;  // below 2^27 tiles times key heads of one sequence
-    at.hc = (int)(in / tiles);
-    at.t = at.s.t0 + in - at.hc * tiles;
-    return u - (at.t - at.s.t0);
+    const uint32_t in = (uint32_t)(u - x), part = at.s.t1 - at.s.t0 + kPartCost;  // below 2^27 tiles times key heads
+    at.hc = (int)(in / part);
+    const uint32_t off = in - at.hc * part, tile = off > kPartCost ? off - kPartCost : 0;
+    at.t = at.s.t0 + tile;
+    at.pos = u - off + kPartCost + tile;
+    return u - off;
   };
 
   // This block's stretch of the line, and this warp's.  Where every part of a sequence is short, blocks
@@ -767,27 +775,27 @@ __global__ void __launch_bounds__(P::WARPS * 32)
   const bool whole = longest <= WARPS * a.whole_tiles;
   const unsigned long long want = whole ? (unsigned long long)live_seqs * hcs : div64(total, WARPS * a.min_tiles) + 1;
   const unsigned blocks = want < gridDim.x ? (unsigned)want : gridDim.x;
-  const unsigned long long share = div64(total + blocks - 1, blocks);  // tiles per block
+  const unsigned long long share = div64(total + blocks - 1, blocks);  // places per block
   unsigned long long lo = share * blockIdx.x, hi = min(lo + share, total);
   if (lo >= total) return;
   if (whole) {  // the parts that begin in the stretch
     Walk<KT> x;
     unsigned long long s0 = locate(lo, x);
-    if (s0 != lo) lo = s0 + (x.s.t1 - x.s.t0);
+    if (s0 != lo) lo = s0 + (x.s.t1 - x.s.t0) + kPartCost;
     s0 = locate(hi - 1, x);
-    hi = max(hi, s0 + (x.s.t1 - x.s.t0));
+    hi = max(hi, s0 + (x.s.t1 - x.s.t0) + kPartCost);
     if (lo >= hi) return;
   }
   const uint32_t each = ((uint32_t)(hi - lo) + WARPS - 1) / WARPS;
   const unsigned long long wlo = min(lo + w * each, hi), whi = min(wlo + each, hi);
 
-  if (wlo < whi) {
+  Walk<KT> at;  // where the softmax is
+  at.pos = whi;
+  if (wlo < whi) locate(wlo, at);
+  if (at.pos < whi) {
     P path;
-    Walk<KT> at;  // where the softmax is
-    locate(wlo, at);
     Walk<KT> ahead = at;  // where the copies are
-    const uint32_t count = (uint32_t)(whi - wlo);
-    uint32_t issued = 0, stage_in = 0, stage_out = 0, parity = 0;
+    uint32_t stage_in = 0, stage_out = 0, parity = 0;
     // Lane i looks up the page of the i-th box of the next tile to issue, a tile early.
     const int boxes = a.page_tiles ? 1 : KT / a.box_rows;
     uint32_t id = 0, slot = 0, span0 = 0, span1 = 0;
@@ -802,7 +810,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
     };
     look();
     auto issue = [&]() {
-      if (issued < count) {
+      if (ahead.pos < whi) {
         const bool bad = live && id >= a.kv.n_pages;
         if (bad) atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
         if constexpr (P::RING) {
@@ -834,17 +842,14 @@ __global__ void __launch_bounds__(P::WARPS * 32)
           }
           stage_in = stage_in + 1 == P::STAGES ? 0 : stage_in + 1;
         }
-        issued++;
-        if (issued < count) {
-          ahead.next(a, hcs);
-          look();
-        }
+        ahead.next(a, hcs);
+        if (ahead.pos < whi) look();
       }
     };
     for (int i = 0; i < P::STAGES - 1; i++) issue();
     uint32_t part_t = at.t;  // where this warp's share of the current sequence part begins
     path.begin(a, at.b, at.hc);
-    for (uint32_t i = 0; i < count; i++) {
+    for (bool more = true; more;) {
       issue();
       if constexpr (P::RING) {
         char* st = ring + stage_out * P::STAGE_BYTES;
@@ -868,7 +873,8 @@ __global__ void __launch_bounds__(P::WARPS * 32)
         }
       }
       const bool ends = at.t + 1 == at.s.t1;
-      if (ends || i + 1 == count) {
+      more = at.pos + 1 + (ends ? kPartCost : 0) < whi;
+      if (ends || !more) {
         const bool starts = part_t == at.s.t0;
         const int which = starts ? 1 : 0;
         float* rec = recs + (w * 2 + which) * rf;
@@ -885,18 +891,19 @@ __global__ void __launch_bounds__(P::WARPS * 32)
           }
           __syncwarp();
         } else if (lane == 0) {
-          seg_id[w * 2 + which] = (long long)(wlo + i) - (long long)(at.t - at.s.t0);
+          seg_id[w * 2 + which] = (long long)at.pos - (long long)(at.t - at.s.t0) - kPartCost;
           seg_b[w * 2 + which] = at.b;
           seg_hc[w * 2 + which] = at.hc;
           seg_tiles[w * 2 + which] = at.s.t1 - at.s.t0;
         }
-        if (i + 1 < count) {
+        if (more) {
           at.next(a, hcs);
           part_t = at.t;
           path.begin(a, at.b, at.hc);
         }
       } else {
         at.t++;
+        at.pos++;
       }
     }
   }
@@ -917,7 +924,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
     left &= left - 1;
     const uint32_t mine = used & (left ? (1u << (__ffs(left) - 1)) - 1 : 0xffffffffu) & ~((1u << r0) - 1);
     const HeadPart hp = head_part(a, seg_hc[r0]);
-    const unsigned long long u0 = seg_id[r0], u1 = u0 + seg_tiles[r0];
+    const unsigned long long u0 = seg_id[r0] + kPartCost, u1 = u0 + seg_tiles[r0];  // its tiles
     const bool before = u0 < lo, open = before || u1 > hi;
     any_open |= open;
     if (open && tid == 0) {
