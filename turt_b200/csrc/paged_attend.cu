@@ -166,6 +166,7 @@ __device__ __forceinline__ void store_head(const AttendArgs& a, int b, int head,
 template <typename T>
 __device__ __noinline__ void attend_plain(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
   const PagedLayout& kv = a.kv;
+  constexpr int AT_ONCE = 4;
   const int lane = threadIdx.x & 31, dim = kv.dim;
   const HeadPart hp = head_part(a, hc);
   for (int g = 0; g < a.part; g++) {
@@ -177,24 +178,51 @@ __device__ __noinline__ void attend_plain(const AttendArgs& a, int b, int hc, ui
       q[i] = head && lane + 32 * i < dim ? qh[lane + 32 * i] * a.scale : 0.f;
       o[i] = 0.f;
     }
-    for (uint32_t j = j0; head && j < j1; j++) {
-      const uint32_t pg = page_of(a, j), id = kv.table[(size_t)b * kv.max_pages + pg];
-      if (id >= kv.n_pages) continue;  // flagged where the tile was opened
-      const size_t off = (size_t)id * kv.page_stride + (size_t)hp.kv * kv.head_stride +
-                         (size_t)(j - pg * kv.page_size) * kv.slot_stride;
-      const T *kr = (const T*)a.kc + off, *vr = (const T*)a.vc + off;
-      float s = 0.f;
+    for (uint32_t j = j0; head && j < j1; j += AT_ONCE) {
+      // lanes 0 .. AT_ONCE - 1 look up a position each; a page out of range was flagged where the tile was opened
+      size_t off = ~(size_t)0;
+      if (lane < AT_ONCE && j + lane < j1) {
+        const uint32_t pg = page_of(a, j + lane), id = kv.table[(size_t)b * kv.max_pages + pg];
+        if (id < kv.n_pages)
+          off = (size_t)id * kv.page_stride + (size_t)hp.kv * kv.head_stride +
+                (size_t)(j + lane - pg * kv.page_size) * kv.slot_stride;
+      }
+      size_t at[AT_ONCE];
+      float s[AT_ONCE], v[AT_ONCE][8];
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (lane + 32 * i < dim) s += q[i] * to_f32(kr[lane + 32 * i]);
-      s = warp_sum(s);
-      const float top = fmaxf(m, s), f = top == -INFINITY ? 1.f : exp2f(m - top);
-      const float p = s == -INFINITY ? 0.f : exp2f(s - top);
+      for (int x = 0; x < AT_ONCE; x++) {
+        at[x] = __shfl_sync(0xffffffffu, off, x);
+        s[x] = 0.f;
+        if (at[x] == ~(size_t)0) continue;
+        const T *kr = (const T*)a.kc + at[x], *vr = (const T*)a.vc + at[x];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (lane + 32 * i < dim) {
+            s[x] += q[i] * to_f32(kr[lane + 32 * i]);
+            v[x][i] = to_f32(vr[lane + 32 * i]);
+          }
+      }
+      float top = m;
+#pragma unroll
+      for (int x = 0; x < AT_ONCE; x++) {
+        s[x] = warp_sum(s[x]);
+        if (at[x] == ~(size_t)0) s[x] = -INFINITY;
+        top = fmaxf(top, s[x]);
+      }
+      const float f = top == -INFINITY ? 1.f : exp2f(m - top);
       m = top;
-      l = l * f + p;
+      l *= f;
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (lane + 32 * i < dim) o[i] = o[i] * f + p * to_f32(vr[lane + 32 * i]);
+      for (int i = 0; i < 8; i++) o[i] *= f;
+#pragma unroll
+      for (int x = 0; x < AT_ONCE; x++) {
+        if (s[x] == -INFINITY) continue;
+        const float p = exp2f(s[x] - top);
+        l += p;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (lane + 32 * i < dim) o[i] += p * v[x][i];
+      }
     }
     float* r = rec + g * (dim + 2);
     if (lane == 0) {
@@ -216,7 +244,7 @@ __device__ __noinline__ void attend_plain(const AttendArgs& a, int b, int hc, ui
 // ------------------------------------------------------------------------------- any layout
 template <typename T>
 struct PathPlain {
-  static constexpr int KT = 16, WARPS = 8, STAGES = 1, STAGE_BYTES = 0;
+  static constexpr int KT = 16, WARPS = 8, STAGES = 1, STAGE_BYTES = 0, BLOCKS = 2;
   static constexpr bool RING = false;
   __device__ void begin(const AttendArgs&, int, int) {}
   __device__ void tile(const AttendArgs&, char*, uint32_t) {}
@@ -227,7 +255,7 @@ struct PathPlain {
 
 // -------------------------------------------------------------- 16-bit caches: tensor cores
 //
-// A tile is 16 positions.  S = Q K^T and O += P V are m16n8k16 products with the heads of the group
+// A tile is 16 or 32 positions.  S = Q K^T and O += P V are m16n8k16 products with the heads of the group
 // (8 at most) as rows.  Only the cache is 16-bit: q and the weights p are fp32 and go in as a sum of
 // 16-bit parts, one part in rows 0-7 and the next in rows 8-15 of the same product, so the unused
 // half of the rows buys the precision: fp16 takes two parts (22 bits; q scaled per head to [1, 2)
@@ -288,15 +316,17 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
 template <typename T, int KD, bool QUAD>
 struct PathMma {
   using H = Half2<T>;
-  static constexpr int KT = 16, WARPS = 8;
-  static constexpr bool RING = true, SWIZZLE = true;
+  // heads of up to 64 elements: twice the positions, for the work per tile that does not grow with them
+  static constexpr int KT = KD <= 4 ? 32 : 16, WARPS = 8, NB = KT / 8;
+  static constexpr bool RING = true;
   static constexpr bool SPLIT = QUAD && H::THREE;    // parts in rows r, r + 4, r + 8
   static constexpr bool EXTRA = !QUAD && H::THREE;   // a product for the third part
-  // slabs of 16 rows of 128 bytes whose 16-byte units are exchanged (unit ^ row % 8): the eight rows of
-  // an ldmatrix fall into different banks
-  static constexpr int SLAB = 64, SLABS = (KD + 3) / 4, SLAB_BYTES = KT * SLAB * 2;
+  // slabs of KT rows of 128 (64) bytes whose 16-byte units are exchanged (unit ^ row % 8, unit ^ row / 2 % 4):
+  // the eight rows of an ldmatrix fall into different banks
+  static constexpr int SLAB = KD <= 2 ? 32 : 64, SLABS = (KD + 3) / 4, ROW = SLAB * 2, SLAB_BYTES = KT * ROW;
+  static constexpr int SWIZZLE = ROW;
   static constexpr int STAGE_BYTES = 2 * SLABS * SLAB_BYTES;
-  static constexpr int STAGES = SLABS == 2 ? 2 : 4;
+  static constexpr int STAGES = 2, BLOCKS = KD <= 2 ? 2 : 1;  // BLOCKS: resident per SM
 
   uint32_t qa[KD][4], qb[EXTRA ? KD : 1][2];
   float acc[2 * KD][2], m, l, unscale;
@@ -374,40 +404,44 @@ struct PathMma {
   }
 
   __device__ void tile(const AttendArgs&, char* st, uint32_t ok) {
-    const int lane = threadIdx.x & 31, c = (lane & 3) * 2;
-    const uint32_t ks = smem_u32(st) + ((lane & 7) + (lane >> 4) * 8) * 128, ku = (lane >> 3) & 1;
-    const uint32_t vs = smem_u32(st) + SLABS * SLAB_BYTES + (lane & 15) * 128, vu = lane >> 4, sw = lane & 7;
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-    float d0[2][4] = {}, d1[2][4] = {};
+    const int lane = threadIdx.x & 31, c = (lane & 3) * 2, sw = KD <= 2 ? (lane >> 1) & 3 : lane & 7;
+    const uint32_t ks = smem_u32(st) + ((lane & 7) + (lane >> 4) * 8) * ROW, ku = (lane >> 3) & 1;
+    const uint32_t vs = smem_u32(st) + SLABS * SLAB_BYTES + (lane & 15) * ROW, vu = lane >> 4;
+    float s[NB][2];
 #pragma unroll
-    for (int k = 0; k < KD; k++) {
-      uint32_t b[4];
-      ldmatrix4(b, ks + k / 4 * SLAB_BYTES + (((k % 4 * 2 + ku) ^ sw) << 4));
-      H::mma(d0[0], qa[k], b[0], b[1], d0[0]);
-      H::mma(d0[1], qa[k], b[2], b[3], d0[1]);
-      if constexpr (EXTRA) {
-        const uint32_t low[4] = {qb[k][0], 0, qb[k][1], 0};
-        H::mma(d1[0], low, b[0], b[1], d1[0]);
-        H::mma(d1[1], low, b[2], b[3], d1[1]);
+    for (int h = 0; h < NB / 2; h++) {
+      float d0[2][4] = {}, d1[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < KD; k++) {
+        uint32_t b[4];
+        ldmatrix4(b, ks + h * 16 * ROW + k / 4 * SLAB_BYTES + (((k % 4 * 2 + ku) ^ sw) << 4));
+        H::mma(d0[0], qa[k], b[0], b[1], d0[0]);
+        H::mma(d0[1], qa[k], b[2], b[3], d0[1]);
+        if constexpr (EXTRA) {
+          const uint32_t low[4] = {qb[k][0], 0, qb[k][1], 0};
+          H::mma(d1[0], low, b[0], b[1], d1[0]);
+          H::mma(d1[1], low, b[2], b[3], d1[1]);
+        }
       }
-    }
-    float s[2][2];
-#pragma unroll
-    for (int n = 0; n < 2; n++)
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        float x = d0[n][i] + (d0[n][2 + i] + (EXTRA ? d1[n][i] : 0.f));
-        if constexpr (SPLIT) x += __shfl_xor_sync(0xffffffffu, x, 16);
-        s[n][i] = H::THREE ? x : x * unscale;
-      }
-    if (ok != 0xFFFF) {
 #pragma unroll
       for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          float x = d0[n][i] + (d0[n][2 + i] + (EXTRA ? d1[n][i] : 0.f));
+          if constexpr (SPLIT) x += __shfl_xor_sync(0xffffffffu, x, 16);
+          s[2 * h + n][i] = H::THREE ? x : x * unscale;
+        }
+    }
+    if (ok != 0xFFFFFFFFu >> (32 - KT)) {
+#pragma unroll
+      for (int n = 0; n < NB; n++)
 #pragma unroll
         for (int i = 0; i < 2; i++)
           if (!((ok >> (n * 8 + c + i)) & 1)) s[n][i] = -INFINITY;
     }
-    float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+    float top = fmaxf(s[0][0], s[0][1]);
+#pragma unroll
+    for (int n = 1; n < NB; n++) top = fmaxf(top, fmaxf(s[n][0], s[n][1]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     if (__any_sync(0xffffffffu, top > m + kLazy)) {
@@ -417,24 +451,36 @@ struct PathMma {
 #pragma unroll
       for (int j = 0; j < 2 * KD; j++) acc[j][0] *= f, acc[j][1] *= f;
     }
-    uint32_t pa[4], pb[4] = {0, 0, 0, 0};
+    const float from = m == -INFINITY ? 0.f : m;
+    uint32_t pa[NB / 2][4], pb[NB / 2][4] = {};
 #pragma unroll
-    for (int n = 0; n < 2; n++) {
-      const float u = exp2_of(s[n][0], m), v = exp2_of(s[n][1], m);
+    for (int n = 0; n < NB; n++) {
+      const float u = exp2f(s[n][0] - from), v = exp2f(s[n][1] - from);
       l += u + v;
-      parts(u, v, pa[2 * n], pa[2 * n + 1], pb[2 * n]);
+      uint32_t(&x)[4] = pa[n / 2];
+      parts(u, v, x[n % 2 * 2], x[n % 2 * 2 + 1], pb[n / 2][n % 2 * 2]);
     }
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < KD; j++) {
-      uint32_t b[4];
-      ldmatrix4_trans(b, vs + j / 4 * SLAB_BYTES + (((j % 4 * 2 + vu) ^ sw) << 4));
+      float d[2][4];
+#pragma unroll
+      for (int h = 0; h < NB / 2; h++) {
+        uint32_t b[4];
+        ldmatrix4_trans(b, vs + h * 16 * ROW + j / 4 * SLAB_BYTES + (((j % 4 * 2 + vu) ^ sw) << 4));
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          if (h == 0)
+            H::mma(d[i], pa[h], b[2 * i], b[2 * i + 1], zero);
+          else
+            H::mma(d[i], pa[h], b[2 * i], b[2 * i + 1], d[i]);
+          if constexpr (EXTRA) H::mma(d[i], pb[h], b[2 * i], b[2 * i + 1], d[i]);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        float d[4];
-        H::mma(d, pa, b[2 * i], b[2 * i + 1], zero);
-        if constexpr (EXTRA) H::mma(d, pb, b[2 * i], b[2 * i + 1], d);
-        acc[2 * j + i][0] += d[0] + d[2];
-        acc[2 * j + i][1] += d[1] + d[3];
+        acc[2 * j + i][0] += d[i][0] + d[i][2];
+        acc[2 * j + i][1] += d[i][1] + d[i][3];
       }
     }
   }
@@ -484,11 +530,12 @@ struct PathFma {
   static constexpr int VE = 16 / (int)sizeof(T), KPW = 32 / LPR;
   static constexpr int KT = LPR <= 16 ? 16 : CPL == 1 ? 8 : 4, R = KT / KPW;
   static constexpr int WARPS = 8;
-  static constexpr bool RING = true, SWIZZLE = false;
+  static constexpr bool RING = true;
+  static constexpr int SWIZZLE = 0;
   static constexpr int SLAB = LPR * CPL * VE, SLABS = 1, PITCH = SLAB * (int)sizeof(T), SLAB_BYTES = KT * PITCH;
   static constexpr int TILE_BYTES = 2 * SLAB_BYTES;
   static constexpr int STAGE_BYTES = TILE_BYTES + (KT * GT * 4 + 127) / 128 * 128;
-  static constexpr int STAGES = TILE_BYTES >= 8192 ? 2 : 4;
+  static constexpr int STAGES = 2, BLOCKS = TILE_BYTES < 8192 && GT <= 4 ? 2 : 1;
   static constexpr int V = R * GT, NV = V > LPR ? V / LPR : 1;  // scores per lane
   static constexpr int SAME = LPR / GT;                         // lanes of a row with scores of one head
   static constexpr int COPIES = V < LPR ? LPR / V : 1;          // lanes of a row with the same score
@@ -656,7 +703,7 @@ constexpr size_t ring_bytes() {
 }
 
 template <typename P>
-__global__ void __launch_bounds__(P::WARPS * 32)
+__global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
     k_paged_attend(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v) {
   constexpr int KT = P::KT, WARPS = P::WARPS, THREADS = WARPS * 32;
@@ -821,7 +868,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
           while (lost) {
             const int x = __ffs(lost) - 1;
             lost &= lost - 1;
-            ok &= ~(((1u << a.box_rows) - 1) << (x * a.box_rows));
+            ok &= ~((0xFFFFFFFFu >> (32 - a.box_rows)) << (x * a.box_rows));
           }
           char* st = ring + stage_in * P::STAGE_BYTES;
           uint64_t* bar = &bars[stage_in * 2];
@@ -856,7 +903,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
         mbar_wait(&bars[stage_out * 2], parity, a.flags, kWaitSite);
         __syncwarp();
         const uint32_t ok = (uint32_t)bars[stage_out * 2 + 1];
-        if (ok != (1u << KT) - 1) {
+        if (ok != 0xFFFFFFFFu >> (32 - KT)) {
           // what the cache holds behind a sequence's end may be NaN, and 0 * NaN is not 0
           constexpr int ROW = P::SLAB_BYTES / KT;
           for (int e = lane * 16; e < P::SLABS * P::SLAB_BYTES; e += 512)
@@ -1018,7 +1065,7 @@ __global__ void __launch_bounds__(P::WARPS * 32)
 }
 
 // Tensor map of a paged cache: [page][head][slot][dim], boxes of `rows` slots x `cols` elements.
-int cache_map(CUtensorMap* map, const void* base, int dtype, const PagedLayout& kv, int cols, int rows, bool swizzle) {
+int cache_map(CUtensorMap* map, const void* base, int dtype, const PagedLayout& kv, int cols, int rows, int swizzle) {
   const TensorMapEncode enc = tensor_map_encode();
   if (!enc) {
     set_error("cuTensorMapEncodeTiled entry point unavailable");
@@ -1033,7 +1080,9 @@ int cache_map(CUtensorMap* map, const void* base, int dtype, const PagedLayout& 
                          : dtype == TURT_CACHE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                          4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                         swizzle == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                         : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                         : CU_TENSOR_MAP_SWIZZLE_NONE,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed (code " + std::to_string((int)r) + ")");
@@ -1047,19 +1096,19 @@ int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
   static std::atomic<uint64_t> done{0};
   a.part = part;
   a.chunks = (a.group + part - 1) / part;
-  a.min_tiles = 2;
-  a.whole_tiles = 4;
+  a.min_tiles = std::max(1, 32 / P::KT);
+  a.whole_tiles = 64 / P::KT;
   a.box_rows = P::KT;
   a.page_tiles = 0;
   CUtensorMap tm_k{}, tm_v{};
   if constexpr (P::RING) {
-    // a tile is one box, two half ones, or (page sizes that neither divides) what a page has of it
+    // a tile is one box or several (of 8 rows at least, the swizzle's period), or, for page sizes that
+    // these do not divide, what a page has of it
     const int ps = (int)a.kv.page_size;
-    if (ps % P::KT != 0) {
-      if (P::KT >= 8 && ps % (P::KT / 2) == 0)
-        a.box_rows = P::KT / 2;
-      else
-        a.page_tiles = (ps + P::KT - 1) / P::KT;
+    while (a.box_rows > (P::SWIZZLE ? 8 : 4) && ps % a.box_rows) a.box_rows /= 2;
+    if (ps % a.box_rows) {
+      a.box_rows = P::KT;
+      a.page_tiles = (ps + P::KT - 1) / P::KT;
     }
     RC(cache_map(&tm_k, a.kc, a.dtype, a.kv, P::SLAB, a.box_rows, P::SWIZZLE));
     RC(cache_map(&tm_v, a.vc, a.dtype, a.kv, P::SLAB, a.box_rows, P::SWIZZLE));
@@ -1069,13 +1118,7 @@ int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
   const size_t rec = (size_t)P::WARPS * 2 * rec_floats(part, a.kv.dim) * 4, smem = ring_bytes<P>() + rec + 1024;
   RC(smem_attr_per_device(done, k_paged_attend<P>, 218 * 1024));
   TURT_REQUIRE(smem <= 218 * 1024, "paged_attention: shared memory");
-  static std::atomic<int> regs{0};
-  if (!regs.load(std::memory_order_relaxed)) {
-    cudaFuncAttributes at;
-    TURT_CHECK_CUDA(cudaFuncGetAttributes(&at, k_paged_attend<P>));
-    regs.store(at.numRegs, std::memory_order_relaxed);
-  }
-  const int per_sm = smem <= 103 * 1024 && regs.load(std::memory_order_relaxed) <= 128 ? 2 : 1;
+  const int per_sm = smem <= 104 * 1024 ? P::BLOCKS : 1;
   const int grid = std::min(kMaxBlocks, sms * per_sm);
   TURT_CHECK_CUDA(launch_pdl(k_paged_attend<P>, dim3(grid), dim3(P::WARPS * 32), smem, ctx->stream, a, tm_k, tm_v));
   TURT_LAUNCH_CHECK();
@@ -1114,7 +1157,7 @@ int attend_mma(turt_ctx* ctx, const AttendArgs& a) {
 template <typename T>
 int attend_typed(turt_ctx* ctx, const AttendArgs& a) {
   const int dim = a.kv.dim;
-  if (!in_boxes<T>(a)) return attend_launch<PathPlain<T>>(ctx, a, 1);
+  if (!in_boxes<T>(a)) return attend_launch<PathPlain<T>>(ctx, a, std::min(a.group, kGroup));
   if constexpr (sizeof(T) == 4) {
     if (dim <= 32) return attend_fma<T, 8, 1, 8>(ctx, a);
     if (dim <= 64) return attend_fma<T, 16, 1, 8>(ctx, a);
