@@ -160,80 +160,101 @@ __device__ __forceinline__ void store_head(const AttendArgs& a, int b, int head,
   if (lane == 0) store_lse(a, b, head, m, l);
 }
 
-// One warp, any layout, head by head: positions [j0, j1) of sequence b into rec (one record of
-// a.part heads).  Lanes take every 32nd element.  The formula as it stands: also what a stretch
-// with infinities or NaN falls back to.
-template <typename T>
+// One warp, any layout: positions [j0, j1) of sequence b into rec (one record of a.part heads), four
+// positions and GH heads at a time.  Lanes take every 32nd element, NI of them.  The formula as it
+// stands: also what a stretch with infinities or NaN falls back to.
+template <typename T, int NI, int GH>
 __device__ __noinline__ void attend_plain(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
-  const PagedLayout& kv = a.kv;
   constexpr int AT_ONCE = 4;
+  const PagedLayout& kv = a.kv;
   const int lane = threadIdx.x & 31, dim = kv.dim;
   const HeadPart hp = head_part(a, hc);
-  for (int g = 0; g < a.part; g++) {
-    float q[8], o[8], m = -INFINITY, l = 0.f;
-    const float* qh = a.q + (size_t)b * a.qs + (size_t)(hp.head + g) * dim;
-    const bool head = g < hp.n;
+  for (int g0 = 0; g0 < a.part; g0 += GH) {
+    float q[GH][NI], o[GH][NI], m[GH], l[GH];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      q[i] = head && lane + 32 * i < dim ? qh[lane + 32 * i] * a.scale : 0.f;
-      o[i] = 0.f;
+    for (int g = 0; g < GH; g++) {
+      const bool head = g0 + g < hp.n;
+      const float* qh = a.q + (size_t)b * a.qs + (size_t)(hp.head + (head ? g0 + g : 0)) * dim;
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        q[g][i] = head && lane + 32 * i < dim ? qh[lane + 32 * i] * a.scale : 0.f;
+        o[g][i] = 0.f;
+      }
+      m[g] = -INFINITY;
+      l[g] = 0.f;
     }
-    for (uint32_t j = j0; head && j < j1; j += AT_ONCE) {
+    for (uint32_t j = j0; j < j1; j += AT_ONCE) {
       // lanes 0 .. AT_ONCE - 1 look up a position each; a page out of range was flagged where the tile was opened
-      size_t off = ~(size_t)0;
+      size_t off = 0;
+      bool there = false;
       if (lane < AT_ONCE && j + lane < j1) {
         const uint32_t pg = page_of(a, j + lane), id = kv.table[(size_t)b * kv.max_pages + pg];
-        if (id < kv.n_pages)
+        there = id < kv.n_pages;
+        if (there)
           off = (size_t)id * kv.page_stride + (size_t)hp.kv * kv.head_stride +
                 (size_t)(j + lane - pg * kv.page_size) * kv.slot_stride;
       }
-      size_t at[AT_ONCE];
-      float s[AT_ONCE], v[AT_ONCE][8];
+      const uint32_t live = __ballot_sync(0xffffffffu, there);
+      float k[AT_ONCE][NI], v[AT_ONCE][NI];
 #pragma unroll
       for (int x = 0; x < AT_ONCE; x++) {
-        at[x] = __shfl_sync(0xffffffffu, off, x);
-        s[x] = 0.f;
-        if (at[x] == ~(size_t)0) continue;
-        const T *kr = (const T*)a.kc + at[x], *vr = (const T*)a.vc + at[x];
+        const size_t at = __shfl_sync(0xffffffffu, off, x);  // position 0 of the cache where there is none
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-          if (lane + 32 * i < dim) {
-            s[x] += q[i] * to_f32(kr[lane + 32 * i]);
-            v[x][i] = to_f32(vr[lane + 32 * i]);
-          }
+        for (int i = 0; i < NI; i++) {
+          const bool in = lane + 32 * i < dim;
+          k[x][i] = in ? to_f32(((const T*)a.kc)[at + lane + 32 * i]) : 0.f;
+          v[x][i] = in ? to_f32(((const T*)a.vc)[at + lane + 32 * i]) : 0.f;
+        }
       }
-      float top = m;
 #pragma unroll
-      for (int x = 0; x < AT_ONCE; x++) {
-        s[x] = warp_sum(s[x]);
-        if (at[x] == ~(size_t)0) s[x] = -INFINITY;
-        top = fmaxf(top, s[x]);
-      }
-      const float f = top == -INFINITY ? 1.f : exp2f(m - top);
-      m = top;
-      l *= f;
+      for (int g = 0; g < GH; g++) {
+        float s[AT_ONCE], top = m[g];
 #pragma unroll
-      for (int i = 0; i < 8; i++) o[i] *= f;
+        for (int x = 0; x < AT_ONCE; x++) {
+          s[x] = 0.f;
 #pragma unroll
-      for (int x = 0; x < AT_ONCE; x++) {
-        if (s[x] == -INFINITY) continue;
-        const float p = exp2f(s[x] - top);
-        l += p;
+          for (int i = 0; i < NI; i++)
+            if (lane + 32 * i < dim) s[x] += q[g][i] * k[x][i];
+          s[x] = warp_sum(s[x]);
+          if (!((live >> x) & 1)) s[x] = -INFINITY;
+          top = fmaxf(top, s[x]);
+        }
+        const float f = top == -INFINITY ? 1.f : exp2f(m[g] - top);
+        m[g] = top;
+        l[g] *= f;
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-          if (lane + 32 * i < dim) o[i] += p * v[x][i];
+        for (int i = 0; i < NI; i++) o[g][i] *= f;
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; x++) {
+          if (s[x] == -INFINITY) continue;  // no weight, whatever the value is
+          const float p = exp2f(s[x] - top);
+          l[g] += p;
+#pragma unroll
+          for (int i = 0; i < NI; i++) o[g][i] += p * v[x][i];
+        }
       }
     }
-    float* r = rec + g * (dim + 2);
-    if (lane == 0) {
-      r[0] = m;
-      r[1] = l;
-    }
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (lane + 32 * i < dim) r[2 + lane + 32 * i] = o[i];
+    for (int g = 0; g < GH; g++) {
+      if (g0 + g >= a.part) continue;
+      float* r = rec + (g0 + g) * (dim + 2);
+      if (lane == 0) {
+        r[0] = m[g];
+        r[1] = l[g];
+      }
+#pragma unroll
+      for (int i = 0; i < NI; i++)
+        if (lane + 32 * i < dim) r[2 + lane + 32 * i] = o[g][i];
+    }
   }
   __syncwarp();
+}
+template <typename T>
+__device__ __forceinline__ void attend_any(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
+  if (a.kv.dim <= 64)
+    attend_plain<T, 2, 4>(a, b, hc, j0, j1, rec);
+  else
+    attend_plain<T, 8, 1>(a, b, hc, j0, j1, rec);
 }
 
 // Paths: how a warp treats the tiles of its stretch.
@@ -249,7 +270,7 @@ struct PathPlain {
   __device__ void begin(const AttendArgs&, int, int) {}
   __device__ void tile(const AttendArgs&, char*, uint32_t) {}
   __device__ void finish(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
-    attend_plain<T>(a, b, hc, j0, j1, rec);
+    attend_any<T>(a, b, hc, j0, j1, rec);
   }
 };
 
@@ -498,7 +519,7 @@ struct PathMma {
         bad |= !(fabsf(acc[j][i]) < INFINITY);
       }
     if (__any_sync(0xffffffffu, bad && r < a.part)) {
-      attend_plain<T>(a, b, hc, j0, j1, rec);
+      attend_any<T>(a, b, hc, j0, j1, rec);
       return;
     }
     if (r < a.part && !(SPLIT && (threadIdx.x & 16))) {
