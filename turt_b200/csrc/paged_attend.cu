@@ -26,7 +26,7 @@ namespace {
 constexpr int kMaxBlocks = 512;           // counters and partial results in the workspace
 constexpr int kPrefix = 1024;             // entries of the tile prefix held in shared memory
 constexpr int kGroup = 8;                 // heads of a group that a warp treats at once, at most
-constexpr int kPartCost = 1;                // what a sequence part costs besides its tiles, in tiles
+constexpr int kPartCost = 2;                // what a sequence part costs besides its tiles, in tiles
 constexpr float kLazy = 8.0f;             // the running max moves when it is this far behind (log2)
 constexpr int kWaitSite = 40;             // reported when a copy's wait runs out
 
@@ -853,6 +853,7 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
     s0 = locate(hi - 1, x);
     hi = max(hi, s0 + (x.s.t1 - x.s.t0) + kPartCost);
     if (lo >= hi) return;
+    lo += kPartCost;  // where its first tile is
   }
   const uint32_t each = ((uint32_t)(hi - lo) + WARPS - 1) / WARPS;
   const unsigned long long wlo = min(lo + w * each, hi), whi = min(wlo + each, hi);
@@ -1118,7 +1119,7 @@ int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
   a.part = part;
   a.chunks = (a.group + part - 1) / part;
   a.min_tiles = std::max(1, 32 / P::KT);
-  a.whole_tiles = 64 / P::KT;
+  a.whole_tiles = std::min(4, 64 / P::KT);
   a.box_rows = P::KT;
   a.page_tiles = 0;
   CUtensorMap tm_k{}, tm_v{};
