@@ -442,6 +442,7 @@ extern "C" int turt_generate_prefill(turt_model* m, const uint32_t* ids, int t, 
     TURT_LAUNCH_CHECK();
   }
   m->dec_len = t;
+  m->dec_logits = m->logits + (size_t)(t - 1) * m->cfg.vocab_size;
   return copy_logits_out(m, m->logits + (size_t)(t - 1) * m->cfg.vocab_size, logits_out);
 }
 
@@ -459,5 +460,13 @@ extern "C" int turt_generate_step(turt_model* m, uint32_t id, int pos, float* lo
   TURT_CHECK_CUDA(cudaGraphLaunch(m->dec_graph, st));
   note_launch(m->dec_graph_kernels);
   m->dec_len = pos + 1;
+  m->dec_logits = dec_bufs(m).logits;
   return copy_logits_out(m, dec_bufs(m).logits, logits_out);
+}
+
+extern "C" int turt_generate_logits(turt_model* m, const float** d_logits) {
+  TURT_REQUIRE(m && d_logits, "generate_logits: null argument");
+  TURT_REQUIRE(m->kcache && m->dec_logits, "generate_logits: nothing generated yet");
+  *d_logits = m->dec_logits;
+  return OK;
 }

@@ -248,6 +248,12 @@ class Model:
         check(lib().turt_generate_step(self._h, int(token), int(pos), ptr(out)))
         return out
 
+    def generate_logits(self) -> int:
+        """Device pointer of the logits that the last generate_prefill / generate_step returned."""
+        p = C.c_void_p()
+        check(lib().turt_generate_logits(self._h, C.byref(p)))
+        return p.value
+
     def clip_grad_norm(self, max_norm: float) -> float:
         n = C.c_double()
         check(lib().turt_clip_grad_norm(self._h, max_norm, C.byref(n)))
