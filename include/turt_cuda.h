@@ -219,7 +219,7 @@ int turt_paged_append(turt_ctx* ctx, const turt_paged_kv* kv, const float* k, si
  * out[b * out_stride ...] hold n_head * head_dim floats per sequence, rotated already.  lse (may be
  * NULL; [batch][n_head]) receives m + ln(sum exp(s_j - m)).  A sequence without positions, or
  * whose scores are all -infinity, gives zeros and -infinity.  Products and sums are in fp32 whatever the cache's type, in an order that
- * depends on the sizes only: equal calls give equal bits.
+ * depends on the sizes and lengths only: equal calls give equal bits.
  * The length of each sequence is read on the device, so a captured call may be replayed with other
  * lengths, page tables and contents.  `workspace` (device, 16-byte aligned, at least
  * turt_paged_attention_workspace bytes for the same sizes) must be zero before its first use
@@ -250,7 +250,8 @@ typedef struct turt_logit_rules {
   int n_masks;
 } turt_logit_rules;
 /* out[r * out_ld + id] = the rules, in the order of the fields above, of logits[r * ld + id] for
- * id < vocab; out = logits with equal pitches works in place.  A masked entry is -infinity
+ * id < vocab (at most 65535 rows); out = logits with equal pitches works in place, other overlaps do
+ * not.  A masked entry is -infinity
  * whatever the logit was; a mask without a set bit leaves nothing.  Ids >= vocab, bias ids that do
  * not increase and masks >= n_masks raise TURT_ERR_RANGE at the next synchronization; the ids are
  * skipped, such a mask counts as none. */

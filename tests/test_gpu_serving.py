@@ -151,6 +151,33 @@ def test_attention(eng, dtype, heads, kvh, dim, page, lens, window):
     check_attend(eng, Cache(lens, kvh, dim, page, dtype, seed=dim), heads, window=window)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [8, 24, 88, 104, 120, 136, 200, 248])
+def test_attention_head_dims(eng, dtype, dim):
+    check_attend(eng, Cache([70, 0, 1, 200], 2, dim, 16, dtype, seed=dim), 2 * (1 + dim % 5))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [1, 2, 4, 7, 8, 12, 16, 33, 40, 1000])
+@pytest.mark.parametrize("dim", [32, 128])
+def test_attention_page_sizes(eng, dtype, page, dim):
+    check_attend(eng, Cache([1, page, page + 1, 150, 0, 2 * page + 3], 2, dim, page, dtype, seed=page), 4)
+    check_attend(eng, Cache([90, 333], 1, dim, page, dtype, seed=page), 3, window=45)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("batch,empty", [(1024, 0), (1025, 1), (3000, 7), (2049, 2)])
+def test_attention_large_batches(eng, dtype, batch, empty):
+    lens = [0 if empty and i % empty == 0 else 1 + (i * 37) % 60 for i in range(batch)]
+    check_attend(eng, Cache(lens, 1, 16, 16, dtype, seed=batch), 2)
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 6, 7, 8, 9, 16, 17])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attention_groups(eng, dtype, group):
+    check_attend(eng, Cache([300, 20], 2, 64, 16, dtype, seed=group), 2 * group)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("lens,heads,kvh", [([30000], 8, 8), ([20001, 3, 9000, 0, 0, 12345], 4, 1), ([1] * 300, 4, 2),
                                             (list(range(0, 700, 7)), 2, 2)])
@@ -402,6 +429,9 @@ def test_append_variants(eng):
     check_append(eng, [40, 7], [5, 7], 8, 2, 64, 16, "bf16", 64, with_q=False)
     check_append(eng, [90001, 130000], [3, 1], 2, 2, 64, 512, "f32", 64, base=5e5)  # far positions
     check_append(eng, list(range(1, 400)), None, 2, 2, 16, 8, "bf16", 16)
+    check_append(eng, [3] * 1100, [(i * 7) % 4 for i in range(1100)], 2, 1, 8, 4, "f16", 8, tail=5)  # many prompts
+    check_append(eng, [900, 901], [900, 700], 3, 3, 24, 16, "f32", 24)  # several rows to a block
+    check_append(eng, [2000], [1999], 40, 8, 128, 16, "bf16", 64)
 
 
 def test_append_bad_pages(eng):

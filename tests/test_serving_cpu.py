@@ -105,7 +105,9 @@ def _rules(rows=4, vocab=100, x=P, ld=100, out=P + 4096, old=100, **kw):
     (dict(repetition=P), "need tokens"), (dict(presence=P), "need tokens"), (dict(frequency=P), "need tokens"),
     (dict(bias_ids=P, bias=P), "bias_start"), (dict(bias_ids=P, bias_start=P), "bias"), (dict(mask=P), "n_masks"),
     (dict(mask=P, n_masks=3), "per row"), (dict(x=None), "null"), (dict(out=None), "null"), (dict(ld=99), "pitch"),
-    (dict(old=99), "pitch"), (dict(out=P, old=104), "in place"), (dict(x=P + 2), "misaligned")])
+    (dict(old=99), "pitch"), (dict(out=P, old=104), "in place"), (dict(x=P + 2), "misaligned"),
+    (dict(tokens=P + 1, token_start=P), "misaligned"), (dict(bias_ids=P, bias=P + 2, bias_start=P), "misaligned"),
+    (dict(mask=P + 3, n_masks=9), "misaligned")])
 def test_rules_refuse(bad, why):
     assert _rules(**bad) == ERR_INVALID and why in last_error()
 

@@ -263,6 +263,20 @@ __device__ __forceinline__ void bring(void* dst, const void* src, uint32_t n, ui
 
 __device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
 
+// Whether `yes` holds for every worker.
+__device__ __forceinline__ bool workers_all(bool yes) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"((uint32_t)yes), "n"(kWorkers)
+      : "memory");
+  return all != 0;
+}
+
 template <bool VEC>
 __global__ void __launch_bounds__(kWorkers + 32, 1)
     k_logit_rules_stream(const __grid_constant__ RuleArgs a, int rows, int slices, int slice, uint32_t slice_mul) {
@@ -321,7 +335,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
       s.s0 = (int)(it - (long)row * slices) * slice - (VEC ? (int)skew_of(in) : 0);
       const int id0 = max(s.s0, 0), id1 = min(s.s0 + slice, V);
       s.word0 = id0 >> 5;
-      if (k >= kRing) mbar_wait(&sh.empty[at], (k / kRing - 1) & 1, a.flags, kWaitSite);
+      if (k >= kRing && !mbar_wait(&sh.empty[at], (k / kRing - 1) & 1, a.flags, kWaitSite)) break;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (id1 > id0) {
@@ -353,7 +367,8 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
   for (long it = first; it < last; it++) {
     const int k = (int)(it - first), at = k % kRing;
     RuleStage& st = sh.ring[at];
-    mbar_wait(&sh.full[at], (k / kRing) & 1, a.flags, kWaitSite);
+    // a wait that ran out is reported; what the stage then holds is not looked at
+    if (!workers_all(mbar_wait(&sh.full[at], (k / kRing) & 1, a.flags, kWaitSite))) break;
     const RuleSlice& s = st.s;
     const int s0 = s.s0, id0 = max(s0, 0), id1 = min(s0 + slice, V);
     if (id1 > id0) {
@@ -552,7 +567,11 @@ extern "C" int turt_logit_rules_apply(turt_ctx* ctx, const float* logits, size_t
   TURT_REQUIRE(rows == 0 || vocab == 0 || (logits && out), "logit_rules: null pointer");
   TURT_REQUIRE(rows <= 1 || (ld >= (size_t)vocab && out_ld >= (size_t)vocab), "logit_rules: pitch below vocab");
   TURT_REQUIRE(out != logits || ld == out_ld, "logit_rules: working in place needs equal pitches");
-  TURT_REQUIRE(((uintptr_t)logits | (uintptr_t)out) % 4 == 0, "logit_rules: misaligned pointer");
+  TURT_REQUIRE(((uintptr_t)logits | (uintptr_t)out | (uintptr_t)r.tokens | (uintptr_t)r.token_start |
+                (uintptr_t)r.generated_start | (uintptr_t)r.repetition | (uintptr_t)r.frequency | (uintptr_t)r.presence |
+                (uintptr_t)r.bias_ids | (uintptr_t)r.bias | (uintptr_t)r.bias_start | (uintptr_t)r.mask |
+                (uintptr_t)r.mask_row) % 4 == 0,
+               "logit_rules: misaligned pointer");
   TURT_REQUIRE(ctx, "null context");
   TURT_CHECK_CUDA(cudaSetDevice(ctx->device));
   if (rows == 0 || vocab == 0) return OK;
