@@ -814,13 +814,12 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
 
   // The first tile at place u of the line or behind it, and where its sequence part begins.
   auto locate = [&](unsigned long long u, Walk<KT>& at) -> unsigned long long {
-    int l = 0, r = n_pre - 1;
-    while (l < r) {
-      const int mid = (l + r + 1) >> 1;
-      if (pre[mid] <= u)
-        l = mid;
-      else
-        r = mid - 1;
+    int l = 0;
+    for (int n = n_pre; n > 1;) {  // the last entry <= u is among l .. l + n - 1: a 32nd of them per step
+      const int piece = (n + 31) / 32, x = l + lane * piece;
+      const int to = (31 - __clz(__ballot_sync(0xffffffffu, x < l + n && pre[x] <= u) | 1)) * piece;
+      l += to;
+      n = min(piece, n - to);
     }
     unsigned long long x = pre[l];
     auto places = [&]() { return at.s.n ? (unsigned long long)(at.s.t1 - at.s.t0 + kPartCost) * hcs : 0; };
@@ -1034,15 +1033,17 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
     }
   }
   if (!any_open) return;
-  __threadfence();
   __syncthreads();
-  if (tid < 2 && open_first[tid] >= 0) s_old[tid] = atomicAdd(&a.counters[open_first[tid]], 1u);
+  if (tid < 2 && open_first[tid] >= 0) {
+    __threadfence();  // the block's results, which the barrier ordered before, then the count
+    s_old[tid] = atomicAdd(&a.counters[open_first[tid]], 1u);
+    __threadfence();  // and the count before anyone's reads of the other blocks' results
+  }
   __syncthreads();
   for (int i = 0; i < 2; i++) {
     const int c0 = open_first[i], parts = open_parts[i];
     if (c0 < 0 || s_old[i] + 1 != (unsigned)parts) continue;
     // the last of its blocks to arrive: every partial result is there
-    __threadfence();
     if (tid == 0) a.counters[c0] = 0;
     const HeadPart hp = head_part(a, seg_hc[open_rec[i]]);
     // Block c0's slot 1, then slot 0 of the next ones, brought to shared memory: one trip to L2 for
