@@ -242,24 +242,33 @@ struct RuleShared {
 // Words between a place and the 16-byte boundary before it.
 __device__ __forceinline__ uint32_t skew_of(const void* p) { return (uint32_t)(reinterpret_cast<uintptr_t>(p) >> 2) & 3; }
 
-// One warp: n words to dst, which lies as far from a 16-byte boundary as src.  Whole 16-byte units go by
-// one bulk copy counted by bar, the words at the ends by hand.
-__device__ __forceinline__ void bring(void* dst, const void* src, uint32_t n, uint64_t* bar, int lane) {
-  uint32_t head = (4 - skew_of(src)) & 3;
-  head = min(head, n);
-  const uint32_t body = (n - head) & ~3u, tail = n - head - body;
-  uint32_t* d = static_cast<uint32_t*>(dst);
-  const uint32_t* s = static_cast<const uint32_t*>(src);
-  if (body && lane == 0) {
-    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(body * 4) : "memory");
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     smem_u32(d + head)),
-                 "l"(s + head), "r"(body * 4), "r"(smem_u32(bar))
-                 : "memory");
+// n words on their way to dst, which lies as far from a 16-byte boundary as src: whole 16-byte units by
+// one bulk copy counted by bar, the words at the ends through the registers of one warp.  They are
+// asked for (ask) well before they are stored (put), or the producer would wait for memory once per array.
+struct Bring {
+  uint32_t* dst;
+  const uint32_t* src;
+  uint32_t head, body, tail, word;
+  __device__ __forceinline__ void ask(void* d, const void* s, uint32_t n, int lane) {
+    dst = static_cast<uint32_t*>(d);
+    src = static_cast<const uint32_t*>(s);
+    head = min((4 - skew_of(s)) & 3, n);
+    body = (n - head) & ~3u;
+    tail = n - head - body;
+    const uint32_t at = lane < 4 ? lane : head + body + lane - 4;
+    if (lane < head || (lane >= 4 && lane - 4 < tail)) word = src[at];
   }
-  if (lane < head) d[lane] = s[lane];
-  if (lane >= 4 && lane - 4 < tail) d[head + body + lane - 4] = s[head + body + lane - 4];
-}
+  __device__ __forceinline__ void put(uint64_t* bar, int lane) const {
+    if (body && lane == 0) {
+      asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(body * 4) : "memory");
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       smem_u32(dst + head)),
+                   "l"(src + head), "r"(body * 4), "r"(smem_u32(bar))
+                   : "memory");
+    }
+    if (lane < head || (lane >= 4 && lane - 4 < tail)) dst[lane < 4 ? lane : head + body + lane - 4] = word;
+  }
+};
 
 __device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
 
@@ -288,7 +297,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
   const long first = items * blockIdx.x / gridDim.x, last = items * (blockIdx.x + 1) / gridDim.x;
   if (tid < kRing) {
     mbar_init(&sh.full[tid], 1);
-    mbar_init(&sh.empty[tid], kWorkers / 32);
+    mbar_init(&sh.empty[tid], 1);
   }
   if (tid < 2) sh.n_list[tid] = 0;
   for (int e = tid; e < kMostIds; e += kWorkers + 32) sh.cnt[e] = 0;
@@ -335,25 +344,32 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
       s.s0 = (int)(it - (long)row * slices) * slice - (VEC ? (int)skew_of(in) : 0);
       const int id0 = max(s.s0, 0), id1 = min(s.s0 + slice, V);
       s.word0 = id0 >> 5;
-      if (k >= kRing && !mbar_wait(&sh.empty[at], (k / kRing - 1) & 1, a.flags, kWaitSite)) break;
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
+      Bring x, tok, ids, val, msk;
+      x.head = x.body = x.tail = tok.head = tok.body = tok.tail = ids.head = ids.body = ids.tail = 0;
+      val.head = val.body = val.tail = msk.head = msk.body = msk.tail = 0;
       if (id1 > id0) {
         // with !VEC a slice may begin anywhere: positions keep the distance to a 16-byte boundary
-        bring(st.x + (VEC ? id0 - s.s0 : skew_of(in + id0)), in + id0, id1 - id0, &sh.full[at], lane);
+        x.ask(st.x + (VEC ? id0 - s.s0 : skew_of(in + id0)), in + id0, id1 - id0, lane);
         if (s.i1 > s.i0 && (fresh || !sort))
-          bring(st.tokens + skew_of(a.r.tokens + s.i0), a.r.tokens + s.i0, min(s.i1 - s.i0, (uint32_t)kTokenRoom),
-                &sh.full[at], lane);
+          tok.ask(st.tokens + skew_of(a.r.tokens + s.i0), a.r.tokens + s.i0, min(s.i1 - s.i0, (uint32_t)kTokenRoom), lane);
         if (s.b1 > s.b0) {
           const uint32_t n = min(s.b1 - s.b0, (uint32_t)kBiasRoom);
-          bring(st.bias_ids + skew_of(a.r.bias_ids + s.b0), a.r.bias_ids + s.b0, n, &sh.full[at], lane);
-          bring(st.bias + skew_of(a.r.bias + s.b0), a.r.bias + s.b0, n, &sh.full[at], lane);
+          ids.ask(st.bias_ids + skew_of(a.r.bias_ids + s.b0), a.r.bias_ids + s.b0, n, lane);
+          val.ask(st.bias + skew_of(a.r.bias + s.b0), a.r.bias + s.b0, n, lane);
         }
         if (s.masked >= 0) {
           const uint32_t* m = a.r.mask + (size_t)s.masked * ((V + 31) / 32) + s.word0;
-          bring(st.mask + skew_of(m), m, ((id1 - 1) >> 5) - s.word0 + 1, &sh.full[at], lane);
+          msk.ask(st.mask + skew_of(m), m, ((id1 - 1) >> 5) - s.word0 + 1, lane);
         }
       }
+      if (k >= kRing && !mbar_wait(&sh.empty[at], (k / kRing - 1) & 1, a.flags, kWaitSite)) break;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      x.put(&sh.full[at], lane);
+      tok.put(&sh.full[at], lane);
+      ids.put(&sh.full[at], lane);
+      val.put(&sh.full[at], lane);
+      msk.put(&sh.full[at], lane);
       if (lane == 0) st.s = s;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.full[at]);
@@ -434,8 +450,22 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
             }
             workers_sync();
           }
-          for (uint32_t i = sh.bins[bin] + tid; i < sh.bins[bin + 1]; i += kWorkers)
-            count((sh.sorted[i] & kSeen) != 0, sh.sorted[i] & ~kSeen);
+          // the warp's new ids take their places in the list with one atomic
+          const uint32_t end = sh.bins[bin + 1];
+          for (uint32_t i0 = sh.bins[bin] + (tid & ~31); i0 < end; i0 += kWorkers) {
+            uint32_t p = 0;
+            bool fresh = false;
+            if (i0 + lane < end) {
+              const uint32_t y = sh.sorted[i0 + lane];
+              p = (y & ~kSeen) - (uint32_t)s0;
+              fresh = ((y & kSeen) ? atomicAdd(&sh.cnt[p], 1u) : atomicOr(&sh.cnt[p], kSeen)) == 0;
+            }
+            const uint32_t all = __ballot_sync(0xffffffffu, fresh);
+            uint32_t at = 0;
+            if (lane == 0 && all) at = atomicAdd(&sh.n_list[turn & 1], (uint32_t)__popc(all));
+            at = __shfl_sync(0xffffffffu, at, 0);
+            if (fresh) sh.list[at + __popc(all & ((1u << lane) - 1))] = (uint16_t)p;
+          }
         } else {
           for (uint32_t q = tid * 4; q < here + skew; q += kWorkers * 4) {  // ids q - skew .. + 3
             const uint4 u = *reinterpret_cast<const uint4*>(st.tokens + q);
@@ -480,31 +510,21 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
       const uint32_t* mask =
           masked ? st.mask + skew_of(a.r.mask + (size_t)s.masked * ((V + 31) / 32) + s.word0) : nullptr;
       const uint32_t words = ((id1 - 1) >> 5) - s.word0 + 1;
-      float* out = a.out + (size_t)s.row * a.out_ld;
       if (VEC) {
-        for (int e = tid * 4; e < slice; e += kWorkers * 4) {
-          const int id = s0 + e;
-          if (id >= id1) break;
-          float4 y = *reinterpret_cast<const float4*>(x + e);
-          if (masked) {
-            const int from = max(id, 0);
+        if (masked)
+          for (int e = tid * 4; e < slice && s0 + e < id1; e += kWorkers * 4) {
+            const int id = s0 + e, from = max(id, 0);
             const uint32_t wd = (from >> 5) - s.word0, low = mask[wd], high = wd + 1 < words ? mask[wd + 1] : 0;
             const uint32_t open = __funnelshift_r(low, high, from & 31) << (from - id);
+            float4 y = *reinterpret_cast<const float4*>(x + e);
             if (!(open & 1)) y.x = -INFINITY;
             if (!(open & 2)) y.y = -INFINITY;
             if (!(open & 4)) y.z = -INFINITY;
             if (!(open & 8)) y.w = -INFINITY;
+            *reinterpret_cast<float4*>(x + e) = y;
           }
-          if (id >= 0 && id + 4 <= id1) {
-            *reinterpret_cast<float4*>(out + id) = y;
-          } else {
-            if (id >= 0) out[id] = y.x;
-            if (id + 1 >= 0 && id + 1 < id1) out[id + 1] = y.y;
-            if (id + 2 >= 0 && id + 2 < id1) out[id + 2] = y.z;
-            if (id + 3 >= 0 && id + 3 < id1) out[id + 3] = y.w;
-          }
-        }
       } else {
+        float* out = a.out + (size_t)s.row * a.out_ld;
         for (int id = id0 + tid; id < id1; id += kWorkers) {
           float y = x[id - s0];
           if (masked && !((mask[(id >> 5) - s.word0] >> (id & 31)) & 1)) y = -INFINITY;
@@ -512,10 +532,35 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
         }
       }
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // in order before the next copies into this stage
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sh.empty[at]);
+    // what was written here goes out by a bulk store (VEC), or comes in by the next bulk copy
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    workers_sync();
+    if (VEC) {
+      // The stage is free once the store has read it: when the next one is on its way.
+      if (id1 > id0) {
+        float* out = a.out + (size_t)s.row * a.out_ld + id0;
+        const float* x = st.x + (id0 - s0);
+        const uint32_t n = id1 - id0, head = min((4 - skew_of(out)) & 3, n), body = (n - head) & ~3u, tail = n - head - body;
+        if (tid == 0 && body)
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out + head),
+                       "r"(smem_u32(x + head)), "r"(body * 4)
+                       : "memory");
+        if (lane < head && tid < 32) out[lane] = x[lane];
+        if (tid >= 32 && tid - 32 < tail) out[head + body + lane] = x[head + body + lane];
+      }
+      if (tid == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      if (k > 0) {
+        if (tid == 0) {
+          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          mbar_arrive(&sh.empty[(k - 1) % kRing]);
+        }
+      }
+      __syncwarp();
+    } else if (tid == 0) {
+      mbar_arrive(&sh.empty[at]);
+    }
   }
+  if (VEC && tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   if (bad) atomicExch(&a.flags[FLAG_RANGE], RANGE_RULE);
 }
 
