@@ -19,7 +19,8 @@
 namespace turt {
 namespace {
 
-constexpr uint32_t kSeen = 0x80000000u;  // count word: in the prompt; the other bits = times generated
+// Count word: in the prompt, has a bias (k_logit_rules_stream), and times generated.
+constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kTimes = 0x3FFFFFFFu;
 constexpr uint32_t kNoMask = 0xFFFFFFFFu;
 
 struct RuleArgs {
@@ -36,8 +37,8 @@ struct RowRules {
 };
 
 __device__ __forceinline__ float penalise(const RowRules& w, float x, uint32_t c) {
-  if (c) x = x > 0.f ? x / w.rep : x * w.rep;
-  const uint32_t n = c & ~kSeen;
+  if (c & ~kBiased) x = x > 0.f ? x / w.rep : x * w.rep;
+  const uint32_t n = c & kTimes;
   if (n) {
     x -= w.freq * (float)n;
     x -= w.pres;
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
     RuleStage& st = sh.ring[at];
     // a wait that ran out is reported; what the stage then holds is not looked at
     if (!workers_all(mbar_wait(&sh.full[at], (k / kRing) & 1, a.flags, kWaitSite))) break;
-    const RuleSlice& s = st.s;
+    const RuleSlice s = st.s;  // in registers: shared memory is written all the time below
     const int s0 = s.s0, id0 = max(s0, 0), id1 = min(s0 + slice, V);
     if (id1 > id0) {
       float* x = st.x + (VEC ? 0 : (int)skew_of(a.in + (size_t)s.row * a.ld + id0));  // position e = id - s0
@@ -484,26 +485,37 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
         }
         for (uint32_t i = here + tid; i < n_tok; i += kWorkers) count(i >= made, a.r.tokens[s.i0 + i]);
         bad |= most >= (uint32_t)V;
+      }
+      const uint32_t* ids = st.bias_ids + skew_of(a.r.bias_ids + s.b0);
+      const float* val = st.bias + skew_of(a.r.bias + s.b0);
+      const uint32_t n_here = min(n_bias, (uint32_t)kBiasRoom);
+      auto bias_id = [&](uint32_t i) { return i < n_here ? ids[i] : a.r.bias_ids[s.b0 + i]; };
+      // (biases go to the last warps first, ids to the first: few of either keep different warps busy)
+      for (uint32_t i = kWorkers - 1 - tid; i < n_bias; i += kWorkers) {
+        const uint32_t id = bias_id(i);
+        bad |= id >= (uint32_t)V || (s0 <= 0 && i > 0 && bias_id(i - 1) >= id);
+        if (id - (uint32_t)id0 < span) atomicOr(&sh.cnt[id - (uint32_t)s0], kBiased);
+      }
+      if (n_tok || n_bias) {
         workers_sync();
+        // ids with a bias belong to it, the others to the list
+        for (uint32_t i = kWorkers - 1 - tid; i < n_bias; i += kWorkers) {
+          const uint32_t id = bias_id(i), p = id - (uint32_t)s0;
+          if (id - (uint32_t)id0 < span) {
+            x[p] = penalise(s.w, x[p], sh.cnt[p]) + (i < n_here ? val[i] : a.r.bias[s.b0 + i]);
+            sh.cnt[p] = 0;
+          }
+        }
         const uint32_t n = sh.n_list[turn & 1];
         for (uint32_t i = tid; i < n; i += kWorkers) {
-          const uint32_t p = sh.list[i];
-          x[p] = penalise(s.w, x[p], sh.cnt[p]);
-          sh.cnt[p] = 0;
+          const uint32_t p = sh.list[i], c = sh.cnt[p];
+          if (c != 0 && !(c & kBiased)) {
+            x[p] = penalise(s.w, x[p], c);
+            sh.cnt[p] = 0;
+          }
         }
         turn++;
         if (tid == 0) sh.n_list[turn & 1] = 0;
-        workers_sync();
-      }
-      if (n_bias) {
-        const uint32_t* ids = st.bias_ids + skew_of(a.r.bias_ids + s.b0);
-        const float* val = st.bias + skew_of(a.r.bias + s.b0);
-        const uint32_t here = min(n_bias, (uint32_t)kBiasRoom);
-        for (uint32_t i = tid; i < n_bias; i += kWorkers) {
-          const uint32_t id = i < here ? ids[i] : a.r.bias_ids[s.b0 + i];
-          bad |= id >= (uint32_t)V || (s0 <= 0 && i > 0 && (i <= here ? ids[i - 1] : a.r.bias_ids[s.b0 + i - 1]) >= id);
-          if (id - (uint32_t)id0 < span) x[id - s0] += i < here ? val[i] : a.r.bias[s.b0 + i];
-        }
         workers_sync();
       }
       const bool masked = s.masked >= 0;
@@ -511,18 +523,30 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
           masked ? st.mask + skew_of(a.r.mask + (size_t)s.masked * ((V + 31) / 32) + s.word0) : nullptr;
       const uint32_t words = ((id1 - 1) >> 5) - s.word0 + 1;
       if (VEC) {
-        if (masked)
-          for (int e = tid * 4; e < slice && s0 + e < id1; e += kWorkers * 4) {
-            const int id = s0 + e, from = max(id, 0);
-            const uint32_t wd = (from >> 5) - s.word0, low = mask[wd], high = wd + 1 < words ? mask[wd + 1] : 0;
-            const uint32_t open = __funnelshift_r(low, high, from & 31) << (from - id);
-            float4 y = *reinterpret_cast<const float4*>(x + e);
-            if (!(open & 1)) y.x = -INFINITY;
-            if (!(open & 2)) y.y = -INFINITY;
-            if (!(open & 4)) y.z = -INFINITY;
-            if (!(open & 8)) y.w = -INFINITY;
-            *reinterpret_cast<float4*>(x + e) = y;
+        if (masked) {
+          constexpr int TURNS = (kMostIds + kWorkers * 4 - 1) / (kWorkers * 4);
+          uint32_t open[TURNS];
+#pragma unroll
+          for (int k = 0; k < TURNS; k++) {
+            const int e = (k * kWorkers + tid) * 4, id = s0 + e, from = max(id, 0);
+            open[k] = 0xF;
+            if (e < slice && id < id1) {
+              const uint32_t wd = (from >> 5) - s.word0, low = mask[wd], high = wd + 1 < words ? mask[wd + 1] : 0;
+              open[k] = __funnelshift_r(low, high, from & 31) << (from - id);
+            }
           }
+#pragma unroll
+          for (int k = 0; k < TURNS; k++) {
+            if ((open[k] & 0xF) == 0xF) continue;
+            float4* at = reinterpret_cast<float4*>(x + (k * kWorkers + tid) * 4);
+            float4 y = *at;
+            if (!(open[k] & 1)) y.x = -INFINITY;
+            if (!(open[k] & 2)) y.y = -INFINITY;
+            if (!(open[k] & 4)) y.z = -INFINITY;
+            if (!(open[k] & 8)) y.w = -INFINITY;
+            *at = y;
+          }
+        }
       } else {
         float* out = a.out + (size_t)s.row * a.out_ld;
         for (int id = id0 + tid; id < id1; id += kWorkers) {
