@@ -102,6 +102,8 @@ _lock = threading.Lock()
 def lib():
     """The loaded library with every header-declared function typed."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):

@@ -191,8 +191,10 @@ class GpuEngine:
     # ------------------------------------------- paged cache, rules on logits (no reference counterpart)
     def pagedAppend(self, kv, k, kStride, v, vStride, rows, start=None, q=None, qStride=0, qOut=None, qOutStride=0,
                     nHead=0, rotDim=0, base=10000.0):
-        check(self.L.turt_paged_append(self.h, C.byref(kv), k, kStride, v, vStride, q, qStride, qOut, qOutStride, nHead,
-                                       start, rows, rotDim, base))
+        rc = self.L.turt_paged_append(self.h, C.byref(kv), k, kStride, v, vStride, q, qStride, qOut, qOutStride, nHead, start,
+                                      rows, rotDim, base)
+        if rc:
+            check(rc)
 
     def pagedAttentionWorkspace(self, kv, nHead) -> int:
         """Bytes of workspace that pagedAttention needs for these sizes (zeroed before its first use)."""
@@ -203,12 +205,15 @@ class GpuEngine:
     def pagedAttention(self, kv, q, qStride, out, outStride, nHead, workspace, workspaceBytes, scale=None, window=0,
                        lse=None):
         """scale None = 1 / sqrt(head_dim)."""
-        check(self.L.turt_paged_attention(self.h, C.byref(kv), q, qStride, out, outStride, lse, nHead,
-                                          1 / math.sqrt(kv.head_dim) if scale is None else scale, window, workspace,
-                                          workspaceBytes))
+        rc = self.L.turt_paged_attention(self.h, C.byref(kv), q, qStride, out, outStride, lse, nHead,
+                                         kv.head_dim ** -0.5 if scale is None else scale, window, workspace, workspaceBytes)
+        if rc:
+            check(rc)
 
     def logitRules(self, logits, ld, out, outLd, rows, vocab, rules):
-        check(self.L.turt_logit_rules_apply(self.h, logits, ld, out, outLd, rows, vocab, C.byref(rules)))
+        rc = self.L.turt_logit_rules_apply(self.h, logits, ld, out, outLd, rows, vocab, C.byref(rules))
+        if rc:
+            check(rc)
 
 
 class GpuTensor:
