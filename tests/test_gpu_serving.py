@@ -250,17 +250,47 @@ def test_attention_infinities_and_nan(eng, dtype, heads):
     assert torch.isnan(out[2:]).all() and torch.isnan(lse[2]).all()
 
 
-def test_attention_garbage_behind_the_length(eng):
+@pytest.mark.parametrize("dtype,dim,page", [("bf16", 64, 16), ("f32", 64, 8), ("bf16", 60, 16), ("f32", 6, 8), ("f16", 128, 8),
+                                            ("bf16", 64, 4)])
+def test_attention_garbage_behind_the_length(eng, dtype, dim, page):
     """NaN in the slots behind a sequence's end, in unused pages and in the window's past does not reach the result (the
     caches above are NaN there too); page numbers that are out of range outside the window are not read."""
-    c = Cache([100, 61], 2, 64, 16, "bf16")
-    c.table[0, :4] = -1
-    c.table[1, :2] = 99999
-    q = torch.randn(2, 256, device="cuda")
+    c = Cache([100, 61], 2, dim, page, dtype)
+    c.table[0, :71 // page] = -1
+    c.table[1, :32 // page] = 99999
+    q = torch.randn(2, 4 * dim, device="cuda")
     out, lse = attend(eng, c, q, 4, window=29)
     want, wl, tol, ltol = expect(c, q, 4, window=29)
     close(out, want, tol)
     close(lse, wl, ltol)
+
+
+@pytest.mark.parametrize("dtype,dim", [("f32", 6), ("bf16", 60), ("bf16", 64), ("f16", 128), ("f32", 128), ("f32", 200)])
+@pytest.mark.parametrize("page", [3, 8, 16, 21, 64])
+def test_attention_each_bad_page_is_reported(eng, dtype, dim, page):
+    """A bad page anywhere in a sequence raises, its positions are left out, and the others count."""
+    from turt_b200._lib import ERR_RANGE, TurtError
+    c = Cache([200], 1, dim, page, dtype)
+    q = torch.randn(1, 2 * dim, device="cuda")
+    want = None
+    for bad in sorted({0, 1, (200 - 1) // page // 2, (200 - 1) // page}):
+        c.table.copy_(c.table_cpu)
+        c.table[0, bad] = c.n_pages + bad
+        out = torch.empty(1, 2 * dim, device="cuda")
+        space = torch.zeros(eng.pagedAttentionWorkspace(c.kv, 2), dtype=torch.uint8, device="cuda")
+        eng.pagedAttention(c.kv, q.data_ptr(), 2 * dim, out.data_ptr(), 2 * dim, 2, space.data_ptr(), space.numel())
+        with pytest.raises(TurtError) as e:
+            eng.ctx.synchronize()
+        assert e.value.code == ERR_RANGE
+        keep = torch.tensor([j for j in range(200) if j // page != bad])
+        if len(keep):
+            k, v = c.read(c.k, 0, 200)[keep, 0], c.read(c.v, 0, 200)[keep, 0]
+            for h in range(2):
+                p = torch.softmax(k @ q[0, h * dim:(h + 1) * dim].cpu().double() / math.sqrt(dim), 0)
+                want = p @ v
+                # the bound of expect(), at most (dim + 4) 2u 4 sqrt(dim) 5 and (200 + 64) 4u for values below 5
+                close(out[0, h * dim:(h + 1) * dim].cpu(), want, 5 * (2 * (dim + 4) * U2 * 20 * math.sqrt(dim) + 600 * U2))
+    assert want is not None
 
 
 def test_attention_bad_pages_and_lengths(eng):

@@ -191,13 +191,15 @@ __device__ __noinline__ void attend_plain(const AttendArgs& a, int b, int hc, ui
       l[g] = 0.f;
     }
     for (uint32_t j = j0; j < j1; j += AT_ONCE) {
-      // lanes 0 .. AT_ONCE - 1 look up a position each; a page out of range was flagged where the tile was opened
+      // lanes 0 .. AT_ONCE - 1 look up a position each
       size_t off = 0;
       bool there = false;
       if (lane < AT_ONCE && j + lane < j1) {
         const uint32_t pg = page_of(a, j + lane), id = kv.table[(size_t)b * kv.max_pages + pg];
         there = id < kv.n_pages;
-        if (there)
+        if (!there)
+          atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
+        else
           off = (size_t)id * kv.page_stride + (size_t)hp.kv * kv.head_stride +
                 (size_t)(j + lane - pg * kv.page_size) * kv.slot_stride;
       }
@@ -879,7 +881,7 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
     auto look = [&]() {
       tile_span<KT>(a, ahead.t, &span0, &span1);
       const uint32_t j = span0 + lane * a.box_rows;
-      live = lane < boxes && j < ahead.s.n && j + a.box_rows > ahead.s.first;
+      live = P::RING && lane < boxes && j < ahead.s.n && j + a.box_rows > ahead.s.first;
       const uint32_t pg = live ? page_of(a, j) : 0;
       slot = j - pg * a.kv.page_size;
       id = live ? a.kv.table[(size_t)ahead.b * a.kv.max_pages + pg] : 0;
