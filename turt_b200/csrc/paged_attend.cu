@@ -68,6 +68,12 @@ __device__ __forceinline__ float exp2_of(float s, float m) { return exp2f(s - (m
 
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+__device__ __forceinline__ unsigned add_acq_rel(uint32_t* p) {
+  unsigned old;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
+  return old;
+}
+
 __device__ __forceinline__ unsigned long long div64(unsigned long long x, unsigned long long y) {
   return (x | y) >> 32 ? x / y : (unsigned)x / (unsigned)y;
 }
@@ -1044,36 +1050,41 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
   }
   if (!any_open) return;
   __syncthreads();
-  if (tid < 2 && open_first[tid] >= 0) {
-    __threadfence();  // the block's results, which the barrier ordered before, then the count
-    s_old[tid] = atomicAdd(&a.counters[open_first[tid]], 1u);
-    __threadfence();  // and the count before anyone's reads of the other blocks' results
-  }
+  // The block's results, which the barrier orders before, then the count, then anyone's reads of the
+  // other blocks' results.
+  if (tid < 2 && open_first[tid] >= 0) s_old[tid] = add_acq_rel(&a.counters[open_first[tid]]);
   __syncthreads();
-  for (int i = 0; i < 2; i++) {
-    const int c0 = open_first[i], parts = open_parts[i];
-    if (c0 < 0 || s_old[i] + 1 != (unsigned)parts) continue;
-    // the last of its blocks to arrive: every partial result is there
-    if (tid == 0) a.counters[c0] = 0;
-    const HeadPart hp = head_part(a, seg_hc[open_rec[i]]);
-    // Block c0's slot 1, then slot 0 of the next ones, brought to shared memory: one trip to L2 for
-    // all of them where they fit.
-    float* stage = reinterpret_cast<float*>(smem);
-    const int rf4 = rf / 4, most = 2 * WARPS + (int)(ring_bytes<P>() / 4) / rf;  // the ring, and the records behind it
-    float o[8] = {}, top = -INFINITY, sum = 0.f;  // of head w
+  // Where this is the last block to arrive, every partial result is there: block c0's slot 1, then slot 0
+  // of the next ones.  They are brought to shared memory (the ring's, and the records' behind it), one trip
+  // to L2 for all of them where they fit; then a warp joins a head.  Two parts are joined at a time where
+  // there are warps for both.
+  float* stage = reinterpret_cast<float*>(smem);
+  const int rf4 = rf / 4, most = 2 * WARPS + (int)(ring_bytes<P>() / 4) / rf;
+  uint32_t todo = 0;
+  for (int i = 0; i < 2; i++)
+    if (open_first[i] >= 0 && s_old[i] + 1 == (unsigned)open_parts[i]) todo |= 1u << i;
+  while (todo) {
+    const bool both = todo == 3 && 2 * a.part <= WARPS && open_parts[0] + open_parts[1] <= most;
+    const int i0 = both ? 0 : __ffs(todo) - 1, first = open_parts[i0], parts = both ? first + open_parts[1] : first;
+    const int mine = both && w >= WARPS / 2 ? 1 : i0, g = both ? w % (WARPS / 2) : w;
+    const HeadPart hp = head_part(a, seg_hc[open_rec[mine]]);
+    todo = both ? 0 : todo & (todo - 1);
+    float o[8] = {}, top = -INFINITY, sum = 0.f;
     for (int x0 = 0; x0 < parts; x0 += most) {
       const int n = min(most, parts - x0);
       __syncthreads();
 #pragma unroll 8
       for (int e = tid; e < n * rf4; e += THREADS) {
-        const int x = e / rf4, at = (c0 + x0 + x) * 2 + (x0 + x == 0);
-        reinterpret_cast<float4*>(stage)[e] = __ldcg(reinterpret_cast<const float4*>(a.partial + (size_t)at * rf) + e - x * rf4);
+        const int r = e / rf4, x = x0 + r, i = x < first ? i0 : 1, y = x < first ? x : x - first;
+        const int at = (open_first[i] + y) * 2 + (y == 0);
+        reinterpret_cast<float4*>(stage)[e] = __ldcg(reinterpret_cast<const float4*>(a.partial + (size_t)at * rf) + e - r * rf4);
       }
       __syncthreads();
-      if (w < hp.n) {
-        const float* rec = stage + w * (dim + 2);
-        for (int y0 = 0; y0 < n; y0 += 32) {
-          const int ny = min(32, n - y0);
+      if (g < hp.n) {
+        const float* rec = stage + (mine != i0 ? first * rf : 0) + g * (dim + 2);
+        const int count = both ? open_parts[mine] : n;
+        for (int y0 = 0; y0 < count; y0 += 32) {
+          const int ny = min(32, count - y0);
           float m = -INFINITY, l = 0.f;
           if (lane < ny) {
             m = rec[(y0 + lane) * rf];
@@ -1093,7 +1104,11 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
         }
       }
     }
-    if (w < hp.n) store_head(a, seg_b[open_rec[i]], hp.head + w, lane, o, top, sum);
+    if (g < hp.n) store_head(a, seg_b[open_rec[mine]], hp.head + g, lane, o, top, sum);
+    if (tid == 0) {
+      a.counters[open_first[i0]] = 0;
+      if (both) a.counters[open_first[1]] = 0;
+    }
   }
 }
 
