@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
           if (s.row != sorted_row) {
             sorted_row = s.row;
             const uint32_t lead = (uint32_t)(bin * slice - s0);
-            constexpr int PER = kTokenRoom / kWorkers;
+            constexpr int PER = (kTokenRoom + kWorkers - 1) / kWorkers;
             uint32_t mine[PER], rank[PER];
             if (tid <= kSorted) sh.bins[tid] = 0;
             workers_sync();
