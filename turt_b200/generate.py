@@ -96,7 +96,7 @@ class LogitRules:
             raise ValueError(f"expected {rows} bias dicts, got {len(self.bias)}")
         self.penalties = bool((self.repetition != 1).any() or self.frequency.any() or self.presence.any())
         self.active = self.penalties or any(self.bias) or allowed is not None
-        self._bufs = {}
+        self._bufs, self._out = {}, None
 
     def _put(self, name: str, a: np.ndarray) -> int:
         return self._bufs.setdefault(name, _Grown(self.ctx)).put(a)
@@ -132,15 +132,18 @@ class LogitRules:
                 kw.update(mask=self._put("mask", np.packbits(bits, axis=1, bitorder="little").view(np.uint32)),
                           mask_row=self._put("mask_row", u32([0xFFFFFFFF if m is None else next(at) for m in masks])),
                           n_masks=len(some))
-        out = self._put("out", np.empty((self.rows, self.vocab), np.float32)) if "out" not in self._bufs else self._bufs["out"].ptr
-        check(lib().turt_logit_rules_apply(self.ctx.handle, d_logits, self.vocab, out, self.vocab, self.rows, self.vocab,
+        if self._out is None:
+            self._out = self.ctx.buffer(self.rows * self.vocab)
+        check(lib().turt_logit_rules_apply(self.ctx.handle, d_logits, self.vocab, self._out, self.vocab, self.rows, self.vocab,
                                            C.byref(make_logit_rules(**kw))))
-        return self.ctx.download(out, self.rows * self.vocab).reshape(self.rows, self.vocab)
+        return self.ctx.download(self._out, self.rows * self.vocab).reshape(self.rows, self.vocab)
 
     def close(self) -> None:
         for b in self._bufs.values():
             b.free()
-        self._bufs = {}
+        if self._out is not None:
+            self.ctx.free(self._out)
+        self._bufs, self._out = {}, None
 
 
 class Generator:
