@@ -13,7 +13,7 @@
 // positions.
 //
 // Measured on a B200 (changing inputs): 96 sequences of up to 8192, 32 query / 8 key heads of 128, bf16
-// (1.63 GB): 277 us, 5.9 TB/s; one of 131001 (537 MB): 99 us, 5.4 TB/s; 64 of up to 1024, 12 heads of
+// (1.63 GB): 281 us, 5.8 TB/s; one of 131001 (537 MB): 98 us, 5.5 TB/s; 64 of up to 1024, 12 heads of
 // 64, fp32 (204 MB): 41 us, 5.0 TB/s.  Of the last, about 5 us pass before the first tile has arrived
 // (length -> page table -> copy, each a trip to memory) and 4 us in the joins.
 #include <math.h>
