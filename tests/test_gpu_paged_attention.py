@@ -1,0 +1,33 @@
+"""Paged attention where it can go wrong: head sizes crossed with the ways a sequence is cut and joined, inputs
+whose elements differ much in size, values and keys that are not finite.
+
+References and tolerances are test_gpu_serving's (64 bits; derived from the arithmetic) unless a test says
+otherwise.
+"""
+import pytest
+
+torch = pytest.importorskip("torch")
+from test_gpu_serving import Cache, attend, close, eng, expect  # noqa: E402,F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,heads,kvh", [(2, 1, 1), (2, 2, 2), (4, 1, 1), (6, 1, 1), (2, 2, 1), (2, 3, 1), (8, 1, 1), (60, 4, 1),
+                                           (250, 2, 2), (256, 5, 1)])
+def test_head_sizes_and_splits(eng, dtype, dim, heads, kvh):
+    """Sequences that two, three and many blocks share.  The workspace holds what a call of other sizes left."""
+    lens = [600, 2000, 1] if dim < 60 else [2000]
+    space = None
+    for n in (lens, [30000 if dim < 60 else 9000]):
+        c = Cache(n, kvh, dim, 16, dtype, seed=dim)
+        need = max(eng.pagedAttentionWorkspace(c.kv, heads), 1 << 24)
+        if space is None:
+            space = torch.zeros(need, dtype=torch.uint8, device="cuda")
+            other = Cache([20000], 1, 64, 16, "f32", seed=9)
+            attend(eng, other, 1000 * torch.randn(1, 8 * 64, device="cuda"), 8, space=space)
+        q = torch.randn(len(n), heads * dim, generator=torch.Generator().manual_seed(dim)).cuda()
+        out, lse = attend(eng, c, q, heads, space=space)
+        want, wl, tol, ltol = expect(c, q, heads)
+        close(out, want, tol)
+        close(lse, wl, ltol)

@@ -138,8 +138,12 @@ struct Walk {
   }
 };
 
-// A result of part of a sequence: per head m (log2), l and dim unnormalised outputs.
-__host__ __device__ __forceinline__ int rec_floats(int part, int dim) { return (part * (dim + 2) + 3) & ~3; }
+// A result of part of a sequence: per head m (log2), l and dim unnormalised outputs.  Two 16-byte units
+// at least: the join divides by the number of units through a 32-bit reciprocal, which 1 has none of.
+__host__ __device__ __forceinline__ int rec_floats(int part, int dim) {
+  const int n = (part * (dim + 2) + 3) & ~3;
+  return n < 8 ? 8 : n;
+}
 
 __device__ __forceinline__ float weight_of(float m, float l, float top) {
   return m == -INFINITY && l == 0.f ? 0.f : exp2f(m - top);
@@ -1070,7 +1074,7 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
     const HeadPart hp = head_part(a, seg_hc[open_rec[mine]]);
     todo = both ? 0 : todo & (todo - 1);
     const int from = open_first[i0], from1 = open_first[1];
-    const uint32_t mul = 0xFFFFFFFFu / rf4 + 1;  // e / rf4 = umulhi(e, mul), e < 2^16
+    const uint32_t mul = 0xFFFFFFFFu / rf4 + 1;  // e / rf4 = umulhi(e, mul), e < 2^16, rf4 > 1
     float o[8] = {}, top = -INFINITY, sum = 0.f;
     for (int x0 = 0; x0 < parts; x0 += most) {
       const int n = min(most, parts - x0);
