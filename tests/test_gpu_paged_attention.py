@@ -31,3 +31,19 @@ def test_head_sizes_and_splits(eng, dtype, dim, heads, kvh):
         want, wl, tol, ltol = expect(c, q, heads)
         close(out, want, tol)
         close(lse, wl, ltol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ratio", [8, 15, 22, 28])
+@pytest.mark.parametrize("dim,heads", [(16, 1), (64, 4), (128, 8)])
+def test_an_outlier_in_q(eng, dtype, ratio, dim, heads):
+    """One element of q 2^ratio times the others, over a key element of 0: it adds nothing to the bound of a score, which
+    the other elements have to keep."""
+    c = Cache([700, 20], 1, dim, 16, dtype, seed=ratio)
+    c.view(c.k)[..., 5] = 0
+    q = torch.randn(2, heads * dim, generator=torch.Generator().manual_seed(ratio)).cuda()
+    q[:, 5::dim] = 2.0 ** ratio
+    out, lse = attend(eng, c, q, heads)
+    want, wl, tol, ltol = expect(c, q, heads)
+    close(out, want, tol)
+    close(lse, wl, ltol)

@@ -298,9 +298,13 @@ struct PathPlain {
 // A tile is 16 or 32 positions.  S = Q K^T and O += P V are m16n8k16 products with the heads of the group
 // (8 at most) as rows.  Only the cache is 16-bit: q and the weights p are fp32 and go in as a sum of
 // 16-bit parts, one part in rows 0-7 and the next in rows 8-15 of the same product, so the unused
-// half of the rows buys the precision: fp16 takes two parts (22 bits; q scaled per head to [1, 2)
-// by a power of two), bf16 three (24 bits): up to four heads have the second in rows 4-7 and the third
-// in rows 8-11, more heads the third in a product of its own.  The thread that holds row r also holds
+// half of the rows buys the precision.  bf16 takes three parts (24 bits): up to four heads have the second
+// in rows 4-7 and the third in rows 8-11, more heads the third in a product of its own.  fp16 takes two:
+// what the first leaves is at most 2^-11 of the element and goes in multiplied by 2^11, so that it is not
+// lost among fp16's subnormals, and its products come back times 2^-11 in fp32.  Both roundings are to 11
+// bits and signed, which leaves an error of 2^-23 of the element, as long as it is not among the
+// subnormals itself: q is scaled per head by a power of two to a maximum in [2^14, 2^15), so an element is off
+// by 2^-23 of itself or 2^-50 of the largest.  The thread that holds row r also holds
 // row r + 8 (and the one 16 lanes on row r + 4), so the parts of a score meet after a shuffle at most,
 // and the scores are where the next product wants p.  Each tile's product is added to the running
 // output in fp32 outside the tensor cores, whose own accumulation truncates.
@@ -311,6 +315,7 @@ struct Half2;
 template <>
 struct Half2<__half> {
   static constexpr bool THREE = false;
+  static constexpr float UP = 2048.f, DOWN = 1.f / 2048.f;  // the second part's scale
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -326,6 +331,7 @@ struct Half2<__half> {
 template <>
 struct Half2<__nv_bfloat16> {
   static constexpr bool THREE = true;
+  static constexpr float UP = 1.f, DOWN = 1.f;
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -376,7 +382,7 @@ struct PathMma {
   static __device__ __forceinline__ void parts(float u, float v, uint32_t& x, uint32_t& y, uint32_t& z) {
     const uint32_t p0 = H::pack(u, v);
     const float2 f0 = H::unpack(p0);
-    u -= f0.x, v -= f0.y;
+    u = (u - f0.x) * H::UP, v = (v - f0.y) * H::UP;
     const uint32_t p1 = H::pack(u, v);
     x = p0, y = p1;
     if constexpr (H::THREE) {
@@ -422,13 +428,9 @@ struct PathMma {
     if constexpr (!H::THREE) {
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t ex = __float_as_uint(top) >> 23;
-      if (ex >= 1 && ex < 253) {
-        up = __uint_as_float((254 - ex) << 23);
-        unscale = __uint_as_float(ex << 23);
-      } else if (ex >= 253) {
-        unscale = NAN;  // leads to attend_plain
-      }
+      const uint32_t ex = max(__float_as_uint(top) >> 23, 15u);  // (2^-112: a smaller q leaves the scores at 0)
+      up = __uint_as_float((268 - ex) << 23);
+      unscale = ex < 255 ? __uint_as_float((ex - 14) << 23) : NAN;  // NaN leads to attend_plain
     }
 #pragma unroll
     for (int k = 0; k < KD; k++)
@@ -468,7 +470,7 @@ struct PathMma {
       for (int n = 0; n < 2; n++)
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          float x = d0[n][i] + (d0[n][2 + i] + (EXTRA ? d1[n][i] : 0.f));
+          float x = d0[n][i] + (H::THREE ? d0[n][2 + i] + (EXTRA ? d1[n][i] : 0.f) : d0[n][2 + i] * H::DOWN);
           if constexpr (SPLIT) x += __shfl_xor_sync(0xffffffffu, x, 16);
           s[2 * h + n][i] = H::THREE ? x : x * unscale;
         }
@@ -520,8 +522,8 @@ struct PathMma {
       }
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        acc[2 * j + i][0] += d[i][0] + d[i][2];
-        acc[2 * j + i][1] += d[i][1] + d[i][3];
+        acc[2 * j + i][0] += d[i][0] + d[i][2] * H::DOWN;
+        acc[2 * j + i][1] += d[i][1] + d[i][3] * H::DOWN;
       }
     }
   }
