@@ -218,8 +218,10 @@ int turt_paged_append(turt_ctx* ctx, const turt_paged_kv* kv, const float* k, si
  * over j in [max(0, lens[b] - window), lens[b]) (window 0 = all).  q[b * q_stride ...] and
  * out[b * out_stride ...] hold n_head * head_dim floats per sequence, rotated already.  lse (may be
  * NULL; [batch][n_head]) receives m + ln(sum exp(s_j - m)).  A sequence without positions, or
- * whose scores are all -infinity, gives zeros and -infinity.  Products and sums are in fp32 whatever the cache's type, in an order that
- * depends on the sizes and lengths only: equal calls give equal bits.
+ * whose scores are all -infinity, gives zeros and -infinity.  Products and sums are in fp32 whatever the
+ * cache's type; with an fp16 cache q and the weights take part with an error of 2^-23 of each (2^-24: fp32), or
+ * 2^-50 of the largest element of the head's q, 2^-49 of the largest of 16 or 32 neighbouring weights, where
+ * that is more.  Their order depends on the sizes and lengths only: equal calls give equal bits.
  * The length of each sequence is read on the device, so a captured call may be replayed with other
  * lengths, page tables and contents.  `workspace` (device, 16-byte aligned, at least
  * turt_paged_attention_workspace bytes for the same sizes) must be zero before its first use

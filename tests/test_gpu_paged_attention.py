@@ -4,6 +4,8 @@ whose elements differ much in size, values and keys that are not finite.
 References and tolerances are test_gpu_serving's (64 bits; derived from the arithmetic) unless a test says
 otherwise.
 """
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -43,6 +45,31 @@ def test_an_outlier_in_q(eng, dtype, ratio, dim, heads):
     c.view(c.k)[..., 5] = 0
     q = torch.randn(2, heads * dim, generator=torch.Generator().manual_seed(ratio)).cuda()
     q[:, 5::dim] = 2.0 ** ratio
+    out, lse = attend(eng, c, q, heads)
+    want, wl, tol, ltol = expect(c, q, heads)
+    close(out, want, tol)
+    close(lse, wl, ltol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("gap", [8, 12, 16, 20])
+@pytest.mark.parametrize("at", [0, 333, 999])
+@pytest.mark.parametrize("dim,heads", [(32, 1), (64, 4), (128, 8)])
+def test_a_dominant_key_without_value(eng, dtype, gap, at, dim, heads):
+    """One position has nearly all of the weight and a value of 0; the output is what the others add, whose weights are
+    e^-gap of it, and its bound is relative to that."""
+    c = Cache([1000, at % 16 + 5], 1, dim, 16, dtype, seed=gap)
+    k, v = c.view(c.k), c.view(c.v)
+    g = torch.Generator().manual_seed(gap)
+    q = torch.randn(2, heads * dim, generator=g).cuda()
+    q[:, 0::dim] = math.sqrt(dim)
+    for b, n in enumerate(c.lens_l):
+        pages, slots = c._at(b, n)
+        k[pages, slots] *= 2.0 ** -7  # scores next to 0 ..
+        k[pages, slots, :, 0] = 0
+        j = at % 16 if b else at
+        k[pages[j], slots[j], :, 0] = gap  # .. and one of them at `gap`
+        v[pages[j], slots[j]] = 0
     out, lse = attend(eng, c, q, heads)
     want, wl, tol, ltol = expect(c, q, heads)
     close(out, want, tol)

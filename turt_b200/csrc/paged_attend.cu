@@ -304,7 +304,10 @@ struct PathPlain {
 // lost among fp16's subnormals, and its products come back times 2^-11 in fp32.  Both roundings are to 11
 // bits and signed, which leaves an error of 2^-23 of the element, as long as it is not among the
 // subnormals itself: q is scaled per head by a power of two to a maximum in [2^14, 2^15), so an element is off
-// by 2^-23 of itself or 2^-50 of the largest.  The thread that holds row r also holds
+// by 2^-23 of itself or 2^-50 of the largest.  The weights of a tile are scaled per head in the same way, to a
+// maximum in (2^13, 2^14], and the tile's product and sum come back times a power of two when they are added to the
+// running ones: a weight is off by 2^-23 of itself or 2^-49 of its tile's largest, however small that is next
+// to the sequence's.  The thread that holds row r also holds
 // row r + 8 (and the one 16 lanes on row r + 4), so the parts of a score meet after a shuffle at most,
 // and the scores are where the next product wants p.  Each tile's product is added to the running
 // output in fp32 outside the tensor cores, whose own accumulation truncates.
@@ -488,21 +491,30 @@ struct PathMma {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     if (__any_sync(0xffffffffu, top > m + kLazy)) {
-      const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : exp2f(m - to);
+      const float to = fmaxf(m, H::THREE ? top : ceilf(top)), f = to == -INFINITY ? 1.f : exp2f(m - to);
       m = to;
       l *= f;
 #pragma unroll
       for (int j = 0; j < 2 * KD; j++) acc[j][0] *= f, acc[j][1] *= f;
     }
-    const float from = m == -INFINITY ? 0.f : m;
+    // fp16: the tile's own exponent, and the power of two that leads from there to m.  (2^14 is multiplied by:
+    // added to the exponent it would round the small differences that the largest weights come from.)
+    const float from = H::THREE ? (m == -INFINITY ? 0.f : m) : top == -INFINITY ? 0.f : ceilf(top);
+    const float back = H::THREE ? 1.f : top == -INFINITY ? 0.f : exp2f(from - m) * 0x1p-14f;
+    float sum = 0.f;
     uint32_t pa[NB / 2][4], pb[NB / 2][4] = {};
 #pragma unroll
     for (int n = 0; n < NB; n++) {
-      const float u = exp2f(s[n][0] - from), v = exp2f(s[n][1] - from);
-      l += u + v;
+      const float u = exp2f(s[n][0] - from) * (H::THREE ? 1.f : 0x1p14f);
+      const float v = exp2f(s[n][1] - from) * (H::THREE ? 1.f : 0x1p14f);
+      if constexpr (H::THREE)
+        l += u + v;
+      else
+        sum += u + v;
       uint32_t(&x)[4] = pa[n / 2];
       parts(u, v, x[n % 2 * 2], x[n % 2 * 2 + 1], pb[n / 2][n % 2 * 2]);
     }
+    if constexpr (!H::THREE) l += sum * back;
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < KD; j++) {
@@ -522,8 +534,13 @@ struct PathMma {
       }
 #pragma unroll
       for (int i = 0; i < 2; i++) {
-        acc[2 * j + i][0] += d[i][0] + d[i][2] * H::DOWN;
-        acc[2 * j + i][1] += d[i][1] + d[i][3] * H::DOWN;
+        if constexpr (H::THREE) {
+          acc[2 * j + i][0] += d[i][0] + d[i][2];
+          acc[2 * j + i][1] += d[i][1] + d[i][3];
+        } else {
+          acc[2 * j + i][0] += (d[i][0] + d[i][2] * H::DOWN) * back;
+          acc[2 * j + i][1] += (d[i][1] + d[i][3] * H::DOWN) * back;
+        }
       }
     }
   }
