@@ -217,8 +217,9 @@ int turt_paged_append(turt_ctx* ctx, const turt_paged_kv* kv, const float* k, si
  *   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  s_j = scale * q . k_j,  m = max_j s_j
  * over j in [max(0, lens[b] - window), lens[b]) (window 0 = all).  q[b * q_stride ...] and
  * out[b * out_stride ...] hold n_head * head_dim floats per sequence, rotated already.  lse (may be
- * NULL; [batch][n_head]) receives m + ln(sum exp(s_j - m)).  A sequence without positions, or
- * whose scores are all -infinity, gives zeros and -infinity.  Products and sums are in fp32 whatever the
+ * NULL; [batch][n_head]) receives m + ln(sum exp(s_j - m)).  A position whose
+ * score is -infinity has no weight, whatever its value.  A sequence without positions, or whose scores are all
+ * -infinity, gives zeros and -infinity.  Products and sums are in fp32 whatever the
  * cache's type; with an fp16 cache q and the weights take part with an error of 2^-23 of each (2^-24: fp32), or
  * 2^-50 of the largest element of the head's q, 2^-49 of the largest of 16 or 32 neighbouring weights, where
  * that is more.  Their order depends on the sizes and lengths only: equal calls give equal bits.

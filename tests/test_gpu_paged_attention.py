@@ -74,3 +74,50 @@ def test_a_dominant_key_without_value(eng, dtype, gap, at, dim, heads):
     want, wl, tol, ltol = expect(c, q, heads)
     close(out, want, tol)
     close(lse, wl, ltol)
+
+
+NARROW_AND_WIDE = [("f32", 16, 1), ("f32", 64, 3), ("f32", 128, 2), ("f32", 200, 4), ("f32", 60, 8), ("f32", 6, 2), ("f16", 64, 3),
+                   ("f16", 200, 2), ("bf16", 128, 8), ("bf16", 136, 4), ("bf16", 60, 2)]
+
+
+@pytest.mark.parametrize("dtype,dim,heads", NARROW_AND_WIDE)
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_no_weight_whatever_the_value(eng, dtype, dim, heads, value):
+    """Positions with a key at -infinity do not count, be their values infinite or NaN."""
+    c = Cache([50, 700], 1, dim, 16, dtype, seed=dim)
+    q = torch.rand(2, heads * dim, generator=torch.Generator().manual_seed(dim)).cuda() + 0.5
+    out_at = {0: [3, 17, 49], 1: [0, 333, 334, 699]}
+    for b, js in out_at.items():
+        pages, slots = c._at(b, c.lens_l[b])
+        for j in js:
+            c.view(c.k)[pages[j], slots[j]] = -math.inf
+            c.view(c.v)[pages[j], slots[j]] = value
+    out, lse = attend(eng, c, q, heads)
+    # the same sequences without these positions
+    left = {b: [j for j in range(n) if j not in out_at[b]] for b, n in enumerate(c.lens_l)}
+    d = Cache([len(left[0]), len(left[1])], 1, dim, 16, dtype)
+    for src, dst in ((c.k, d.k), (c.v, d.v)):
+        for b in left:
+            pages, slots = c._at(b, c.lens_l[b])
+            d.view(dst)[d._at(b, len(left[b]))] = c.view(src)[pages[left[b]], slots[left[b]]]
+    want, wl, tol, ltol = expect(d, q, heads)
+    close(out, want, tol)
+    close(lse, wl, ltol)
+
+
+@pytest.mark.parametrize("dtype,dim,heads", [x for x in NARROW_AND_WIDE if x[0] != "f16"])
+@pytest.mark.parametrize("size", [1e34, 3e34, 1e35])
+def test_values_near_the_largest(eng, dtype, dim, heads, size):
+    """Values from 1e34 on under scores that rise and fall by 5 (2^7.2) from one 16 positions to the next: sums of 32 or
+    256 of them at a weight of 2^7.2 are past fp32's range, sums of 256 at a weight of 1 are not."""
+    c = Cache([512], 1, dim, 16, dtype, seed=dim)
+    q = torch.zeros(1, heads * dim, device="cuda")
+    q[:, 0::dim] = math.sqrt(dim)
+    pages, slots = c._at(0, 512)
+    c.view(c.k)[pages, slots] = 0
+    c.view(c.k)[pages, slots, :, 0] = (5.0 * ((torch.arange(512) // 16) % 2))[:, None].to(c.k)
+    c.view(c.v)[pages, slots] = (c.view(c.v)[pages, slots].abs() + 1) * size
+    out, lse = attend(eng, c, q, heads)
+    want, wl, tol, ltol = expect(c, q, heads)
+    close(out, want, tol)
+    close(lse, wl, ltol)

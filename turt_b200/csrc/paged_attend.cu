@@ -268,29 +268,37 @@ __device__ __noinline__ void attend_plain(const AttendArgs& a, int b, int hc, ui
   }
   __syncwarp();
 }
-template <typename T>
-__device__ __forceinline__ void attend_any(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
-  if (a.kv.dim <= 64)
-    attend_plain<T, 2, 4>(a, b, hc, j0, j1, rec);
-  else
-    attend_plain<T, 8, 1>(a, b, hc, j0, j1, rec);
+// The running maximum may lie up to kLazy behind, with weights above 1.  Where sums are so large that the joins
+// could take them out of range, they are brought to weights of 1 at most, as the exact maximum gives.
+template <int N, int K>
+__device__ __forceinline__ void below_one(float (&acc)[N][K], float& m, float& l) {
+  bool big = false;
+#pragma unroll
+  for (int i = 0; i < N; i++)
+#pragma unroll
+    for (int k = 0; k < K; k++) big |= fabsf(acc[i][k]) > 0x1p100f;
+  if (!__any_sync(0xffffffffu, big)) return;
+  constexpr float down = 1.f / (1 << (int)kLazy);
+  m += kLazy;
+  l *= down;
+#pragma unroll
+  for (int i = 0; i < N; i++)
+#pragma unroll
+    for (int k = 0; k < K; k++) acc[i][k] *= down;
 }
 
 // Paths: how a warp treats the tiles of its stretch.
-//   begin / tile / finish   the softmax of one part of a sequence; finish leaves its record in rec
+//   begin / tile / finish   the softmax of one part of a sequence; finish leaves its record in rec, or
+//                           returns false where something in it is not finite
 //   A tile lies in its stage of the ring as KT rows of keys and then KT of values, in slabs of SLAB
 //   elements (a slab holds all KT rows); `ok` has a bit for each row that is attended to, and the
 //   value rows without one are zero.
 // ------------------------------------------------------------------------------- any layout
 template <typename T>
-struct PathPlain {
-  static constexpr int KT = 16, WARPS = 8, STAGES = 1, STAGE_BYTES = 0, BLOCKS = 2;
+struct PathPlain {  // attend_plain alone
+  using Type = T;
+  static constexpr int KT = 16, WARPS = 8, STAGES = 1, STAGE_BYTES = 0, BLOCKS = 2, MAX_DIM = 256;
   static constexpr bool RING = false;
-  __device__ void begin(const AttendArgs&, int, int) {}
-  __device__ void tile(const AttendArgs&, char*, uint32_t) {}
-  __device__ void finish(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
-    attend_any<T>(a, b, hc, j0, j1, rec);
-  }
 };
 
 // -------------------------------------------------------------- 16-bit caches: tensor cores
@@ -311,8 +319,7 @@ struct PathPlain {
 // row r + 8 (and the one 16 lanes on row r + 4), so the parts of a score meet after a shuffle at most,
 // and the scores are where the next product wants p.  Each tile's product is added to the running
 // output in fp32 outside the tensor cores, whose own accumulation truncates.
-// Infinities and NaN break the parts (0 * inf): a stretch that ends in a non-finite result is done
-// again by attend_plain.
+// Infinities and NaN break the parts (0 * inf).
 template <typename T>
 struct Half2;
 template <>
@@ -364,10 +371,12 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
 // KD: steps of 16 elements that cover head_dim (a multiple of 8).  QUAD: at most four heads.
 template <typename T, int KD, bool QUAD>
 struct PathMma {
+  using Type = T;
   using H = Half2<T>;
   // heads of up to 64 elements: twice the positions, for the work per tile that does not grow with them
   // (16 / 8 heads of 64, 32 x 4000 positions: 50 us, with tiles of 16 positions 66 us)
   static constexpr int KT = KD <= 4 ? 32 : 16, WARPS = 8, NB = KT / 8;
+  static constexpr int MAX_DIM = KD * 16;
   static constexpr bool RING = true;
   static constexpr bool SPLIT = QUAD && H::THREE;    // parts in rows r, r + 4, r + 8
   static constexpr bool EXTRA = !QUAD && H::THREE;   // a product for the third part
@@ -545,8 +554,9 @@ struct PathMma {
     }
   }
 
-  __device__ void finish(const AttendArgs& a, int b, int hc, uint32_t j0, uint32_t j1, float* rec) {
+  __device__ bool finish(const AttendArgs& a, float* rec) {
     const int r = row(), c = (threadIdx.x & 3) * 2, dim = a.kv.dim;
+    below_one(acc, m, l);
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     bool bad = !(fabsf(l) < INFINITY);
@@ -557,10 +567,7 @@ struct PathMma {
         if constexpr (SPLIT) acc[j][i] += __shfl_xor_sync(0xffffffffu, acc[j][i], 16);
         bad |= !(fabsf(acc[j][i]) < INFINITY);
       }
-    if (__any_sync(0xffffffffu, bad && r < a.part)) {
-      attend_any<T>(a, b, hc, j0, j1, rec);
-      return;
-    }
+    if (__any_sync(0xffffffffu, bad && r < a.part)) return false;
     if (r < a.part && !(SPLIT && (threadIdx.x & 16))) {
       float* x = rec + r * (dim + 2);
       if (c == 0) {
@@ -575,6 +582,7 @@ struct PathMma {
         }
     }
     __syncwarp();
+    return true;
   }
 };
 
@@ -587,9 +595,10 @@ struct PathMma {
 // lane ends with the scores that it turns into weights (no weight is computed twice).
 template <typename T, int LPR, int CPL, int GT>
 struct PathFma {
+  using Type = T;
   static constexpr int VE = 16 / (int)sizeof(T), KPW = 32 / LPR;
   static constexpr int KT = LPR <= 16 ? 16 : CPL == 1 ? 8 : 4, R = KT / KPW;
-  static constexpr int WARPS = 8;
+  static constexpr int WARPS = 8, MAX_DIM = LPR * CPL * VE;
   static constexpr bool RING = true;
   static constexpr int SWIZZLE = 0;
   static constexpr int SLAB = LPR * CPL * VE, SLABS = 1, PITCH = SLAB * (int)sizeof(T), SLAB_BYTES = KT * PITCH;
@@ -724,8 +733,11 @@ struct PathFma {
     }
   }
 
-  __device__ void finish(const AttendArgs& a, int, int, uint32_t, uint32_t, float* rec) {
+  // (Not finite where the formula is: a weight of 0 times an infinite value, weights of up to 2^kLazy times values
+  // near the largest.)
+  __device__ bool finish(const AttendArgs& a, float* rec) {
     const int dim = a.kv.dim;
+    below_one(acc, m, l);
 #pragma unroll
     for (int o = 1; o < SAME; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
 #pragma unroll
@@ -736,6 +748,12 @@ struct PathFma {
 #pragma unroll
         for (int i = 0; i < CPL * VE; i++) acc[g][i] += __shfl_xor_sync(0xffffffffu, acc[g][i], o);
     }
+    bool bad = !(fabsf(l) < INFINITY);
+#pragma unroll
+    for (int g = 0; g < GT; g++)
+#pragma unroll
+      for (int i = 0; i < CPL * VE; i++) bad |= !(fabsf(acc[g][i]) < INFINITY);
+    if (__any_sync(0xffffffffu, bad)) return false;
     if (group() == 0) {
 #pragma unroll
       for (int g = 0; g < GT; g++) {
@@ -753,10 +771,71 @@ struct PathFma {
       }
     }
     __syncwarp();
+    return true;
   }
 };
 
 // ------------------------------------------------------------------------------ the kernel
+// The records of a warp: [0] a part that goes on from the stretch before, [1] one that begins in this stretch.
+struct Records {
+  float* rec;        // [2][rf]
+  int rf;
+  long long* id;     // where on the line the sequence part begins, -1: none
+  int *b, *hc, *tiles;
+};
+
+// Positions of the tiles [t0, t1] of a sequence.
+template <int KT>
+__device__ __forceinline__ uint2 positions(const AttendArgs& a, const Seq& s, uint32_t t0, uint32_t t1) {
+  uint32_t j0, j1, skip;
+  tile_span<KT>(a, t0, &j0, &skip);
+  tile_span<KT>(a, t1, &skip, &j1);
+  return make_uint2(max(s.first, j0), min(s.n, j1));
+}
+
+// At the last tile of a sequence part that this warp sees: its record is the result, or goes to the joins.
+template <int KT>
+__device__ __forceinline__ void end_part(const AttendArgs& a, const Walk<KT>& at, bool starts, bool ends, const Records& r) {
+  const int lane = threadIdx.x & 31, which = starts ? 1 : 0, dim = a.kv.dim;
+  if (starts && ends) {
+    const HeadPart hp = head_part(a, at.hc);
+    for (int g = 0; g < hp.n; g++) {
+      const float* x = r.rec + which * r.rf + g * (dim + 2);
+      for (int d = lane; d < dim; d += 32) store_out(a, at.b, hp.head + g, d, x[2 + d], x[1]);
+      if (lane == 0) store_lse(a, at.b, hp.head + g, x[0], x[1]);
+    }
+    __syncwarp();
+  } else if (lane == 0) {
+    r.id[which] = (long long)at.pos - (long long)(at.t - at.s.t0) - kPartCost;
+    r.b[which] = at.b;
+    r.hc[which] = at.hc;
+    r.tiles[which] = at.s.t1 - at.s.t0;
+  }
+}
+
+// The stretch [at, whi) by attend_plain: any layout, and once more where a path met something that is not
+// finite.  A function of its own, behind the loop over tiles: a call inside that loop made it spill, which cost
+// 16-bit heads of 16 and 32 and eight bf16 heads of 128 per key head half of their rate.
+template <typename P>
+__device__ __noinline__ void attend_stretch(const AttendArgs& a, Walk<P::KT> at, unsigned long long whi, Records r) {
+  const int hcs = a.kv.kv_heads * a.chunks;
+  while (true) {
+    const uint32_t from = at.t, n = (uint32_t)min(whi - at.pos, (unsigned long long)(at.s.t1 - at.t));
+    at.t += n - 1;
+    at.pos += n - 1;
+    const bool starts = from == at.s.t0, ends = at.t + 1 == at.s.t1;
+    const uint2 j = positions<P::KT>(a, at.s, from, at.t);
+    float* rec = r.rec + (starts ? r.rf : 0);
+    if (P::MAX_DIM <= 64 || a.kv.dim <= 64)
+      attend_plain<typename P::Type, 2, 4>(a, at.b, at.hc, j.x, j.y, rec);
+    else
+      attend_plain<typename P::Type, 8, 1>(a, at.b, at.hc, j.x, j.y, rec);
+    end_part(a, at, starts, ends, r);
+    if (at.pos + 1 + (ends ? kPartCost : 0) >= whi) return;
+    at.next(a, hcs);
+  }
+}
+
 template <typename P>
 constexpr size_t ring_bytes() {
   return (size_t)P::WARPS * P::STAGES * (P::STAGE_BYTES + 16);  // stages, then barriers and row bits of each
@@ -900,65 +979,64 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
   at.pos = whi;
   if (wlo < whi) locate(wlo, at);
   if (at.pos < whi) {
-    P path;
-    Walk<KT> ahead = at;  // where the copies are
-    uint32_t stage_in = 0, stage_out = 0, parity = 0;
-    // Lane i looks up the page of the i-th box of the next tile to issue, a tile early.
-    const int boxes = a.page_tiles ? 1 : KT / a.box_rows;
-    uint32_t id = 0, slot = 0, span0 = 0, span1 = 0;
-    bool live = false;
-    auto look = [&]() {
-      tile_span<KT>(a, ahead.t, &span0, &span1);
-      const uint32_t j = span0 + lane * a.box_rows;
-      live = P::RING && lane < boxes && j < ahead.s.n && j + a.box_rows > ahead.s.first;
-      const uint32_t pg = live ? page_of(a, j) : 0;
-      slot = j - pg * a.kv.page_size;
-      id = live ? a.kv.table[(size_t)ahead.b * a.kv.max_pages + pg] : 0;
-    };
-    look();
-    auto issue = [&]() {
-      if (ahead.pos < whi) {
+    const Records mine = {recs + w * 2 * rf, rf, seg_id + w * 2, seg_b + w * 2, seg_hc + w * 2, seg_tiles + w * 2};
+    if constexpr (P::RING) {
+      P path;
+      bool again = false;
+      Walk<KT> ahead = at;  // where the copies are
+      uint32_t stage_in = 0, stage_out = 0, parity = 0;
+      // Lane i looks up the page of the i-th box of the next tile to issue, a tile early.
+      const int boxes = a.page_tiles ? 1 : KT / a.box_rows;
+      uint32_t id = 0, slot = 0, span0 = 0, span1 = 0;
+      bool live = false;
+      auto look = [&]() {
+        tile_span<KT>(a, ahead.t, &span0, &span1);
+        const uint32_t j = span0 + lane * a.box_rows;
+        live = lane < boxes && j < ahead.s.n && j + a.box_rows > ahead.s.first;
+        const uint32_t pg = live ? page_of(a, j) : 0;
+        slot = j - pg * a.kv.page_size;
+        id = live ? a.kv.table[(size_t)ahead.b * a.kv.max_pages + pg] : 0;
+      };
+      look();
+      auto issue = [&]() {
+        if (ahead.pos >= whi) return;
         const bool bad = live && id >= a.kv.n_pages;
         if (bad) atomicExch(&a.flags[FLAG_RANGE], RANGE_PAGE);
-        if constexpr (P::RING) {
-          // rows that are attended to: within the sequence, the window and (one box only) the page
-          const uint32_t lo = ahead.s.first > span0 ? ahead.s.first - span0 : 0, hi = min(ahead.s.n, span1) - span0;
-          uint32_t ok = ((2u << (hi - 1)) - 1) & ~((1u << lo) - 1);
-          uint32_t lost = __ballot_sync(0xffffffffu, bad);
-          while (lost) {
-            const int x = __ffs(lost) - 1;
-            lost &= lost - 1;
-            ok &= ~((0xFFFFFFFFu >> (32 - a.box_rows)) << (x * a.box_rows));
-          }
-          char* st = ring + stage_in * P::STAGE_BYTES;
-          uint64_t* bar = &bars[stage_in * 2];
-          if (lane == 0) {
-            bar[1] = ok;
-            mbar_arrive_expect_tx(bar, 2 * P::SLABS * P::SLAB_BYTES);
-          }
-          __syncwarp();
-          if (lane < boxes) {
-            // a box without a page lies outside the tensor: zeros
-            const int page = live && !bad ? (int)id : (int)a.kv.n_pages, hk = head_part(a, ahead.hc).kv;
-            const uint32_t dst = smem_u32(st) + lane * a.box_rows * (P::SLAB_BYTES / KT);
-#pragma unroll
-            for (int c = 0; c < P::SLABS; c++) {
-              tma_load_4d(dst + c * P::SLAB_BYTES, &tm_k, c * P::SLAB, (int)slot, hk, page, bar);
-              tma_load_4d(dst + (P::SLABS + c) * P::SLAB_BYTES, &tm_v, c * P::SLAB, (int)slot, hk, page, bar);
-            }
-          }
-          stage_in = stage_in + 1 == P::STAGES ? 0 : stage_in + 1;
+        // rows that are attended to: within the sequence, the window and (one box only) the page
+        const uint32_t lo = ahead.s.first > span0 ? ahead.s.first - span0 : 0, hi = min(ahead.s.n, span1) - span0;
+        uint32_t ok = ((2u << (hi - 1)) - 1) & ~((1u << lo) - 1);
+        uint32_t lost = __ballot_sync(0xffffffffu, bad);
+        while (lost) {
+          const int x = __ffs(lost) - 1;
+          lost &= lost - 1;
+          ok &= ~((0xFFFFFFFFu >> (32 - a.box_rows)) << (x * a.box_rows));
         }
+        char* st = ring + stage_in * P::STAGE_BYTES;
+        uint64_t* bar = &bars[stage_in * 2];
+        if (lane == 0) {
+          bar[1] = ok;
+          mbar_arrive_expect_tx(bar, 2 * P::SLABS * P::SLAB_BYTES);
+        }
+        __syncwarp();
+        if (lane < boxes) {
+          // a box without a page lies outside the tensor: zeros
+          const int page = live && !bad ? (int)id : (int)a.kv.n_pages, hk = head_part(a, ahead.hc).kv;
+          const uint32_t dst = smem_u32(st) + lane * a.box_rows * (P::SLAB_BYTES / KT);
+#pragma unroll
+          for (int c = 0; c < P::SLABS; c++) {
+            tma_load_4d(dst + c * P::SLAB_BYTES, &tm_k, c * P::SLAB, (int)slot, hk, page, bar);
+            tma_load_4d(dst + (P::SLABS + c) * P::SLAB_BYTES, &tm_v, c * P::SLAB, (int)slot, hk, page, bar);
+          }
+        }
+        stage_in = stage_in + 1 == P::STAGES ? 0 : stage_in + 1;
         ahead.next(a, hcs);
         if (ahead.pos < whi) look();
-      }
-    };
-    for (int i = 0; i < P::STAGES - 1; i++) issue();
-    uint32_t part_t = at.t;  // where this warp's share of the current sequence part begins
-    path.begin(a, at.b, at.hc);
-    for (bool more = true; more;) {
-      issue();
-      if constexpr (P::RING) {
+      };
+      for (int i = 0; i < P::STAGES - 1; i++) issue();
+      uint32_t part_t = at.t;  // where this warp's share of the current sequence part begins
+      path.begin(a, at.b, at.hc);
+      for (bool more = true; more;) {
+        issue();
         char* st = ring + stage_out * P::STAGE_BYTES;
         mbar_wait(&bars[stage_out * 2], parity, a.flags, kWaitSite);
         __syncwarp();
@@ -978,40 +1056,39 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
           stage_out = 0;
           parity ^= 1;
         }
-      }
-      const bool ends = at.t + 1 == at.s.t1;
-      more = at.pos + 1 + (ends ? kPartCost : 0) < whi;
-      if (ends || !more) {
-        const bool starts = part_t == at.s.t0;
-        const int which = starts ? 1 : 0;
-        float* rec = recs + (w * 2 + which) * rf;
-        uint32_t j0, j1, skip;
-        tile_span<KT>(a, part_t, &j0, &skip);
-        tile_span<KT>(a, at.t, &skip, &j1);
-        path.finish(a, at.b, at.hc, max(at.s.first, j0), min(at.s.n, j1), rec);
-        if (starts && ends) {
-          const HeadPart hp = head_part(a, at.hc);
-          for (int g = 0; g < hp.n; g++) {
-            const float* x = rec + g * (dim + 2);
-            for (int d = lane; d < dim; d += 32) store_out(a, at.b, hp.head + g, d, x[2 + d], x[1]);
-            if (lane == 0) store_lse(a, at.b, hp.head + g, x[0], x[1]);
+        const bool ends = at.t + 1 == at.s.t1;
+        more = at.pos + 1 + (ends ? kPartCost : 0) < whi;
+        if (ends || !more) {
+          const bool starts = part_t == at.s.t0;
+          if (!path.finish(a, mine.rec + (starts ? rf : 0))) {
+            again = true;
+            break;
           }
-          __syncwarp();
-        } else if (lane == 0) {
-          seg_id[w * 2 + which] = (long long)at.pos - (long long)(at.t - at.s.t0) - kPartCost;
-          seg_b[w * 2 + which] = at.b;
-          seg_hc[w * 2 + which] = at.hc;
-          seg_tiles[w * 2 + which] = at.s.t1 - at.s.t0;
+          end_part(a, at, starts, ends, mine);
+          if (more) {
+            at.next(a, hcs);
+            part_t = at.t;
+            path.begin(a, at.b, at.hc);
+          }
+        } else {
+          at.t++;
+          at.pos++;
         }
-        if (more) {
-          at.next(a, hcs);
-          part_t = at.t;
-          path.begin(a, at.b, at.hc);
-        }
-      } else {
-        at.t++;
-        at.pos++;
       }
+      if (again) {
+        // the copies under way land first: the joins use the ring's memory
+        while (stage_out != stage_in) {
+          mbar_wait(&bars[stage_out * 2], parity, a.flags, kWaitSite);
+          if (++stage_out == P::STAGES) {
+            stage_out = 0;
+            parity ^= 1;
+          }
+        }
+        locate(wlo, at);
+        attend_stretch<P>(a, at, whi, mine);
+      }
+    } else {
+      attend_stretch<P>(a, at, whi, mine);
     }
   }
   __syncthreads();
