@@ -814,7 +814,7 @@ __device__ __forceinline__ void end_part(const AttendArgs& a, const Walk<KT>& at
 }
 
 // The stretch [at, whi) by attend_plain: any layout, and once more where a path met something that is not
-// finite.  A function of its own, behind the loop over tiles: a call inside that loop made it spill, which cost
+// finite or a copy that did not arrive in time.  A function of its own, behind the loop over tiles: a call inside that loop made it spill, which cost
 // 16-bit heads of 16 and 32 and eight bf16 heads of 128 per key head half of their rate.
 template <typename P>
 __device__ __noinline__ void attend_stretch(const AttendArgs& a, Walk<P::KT> at, unsigned long long whi, Records r) {
@@ -982,7 +982,7 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
     const Records mine = {recs + w * 2 * rf, rf, seg_id + w * 2, seg_b + w * 2, seg_hc + w * 2, seg_tiles + w * 2};
     if constexpr (P::RING) {
       P path;
-      bool again = false;
+      bool again = false, late = false;  // late: a wait ran out, which is reported
       Walk<KT> ahead = at;  // where the copies are
       uint32_t stage_in = 0, stage_out = 0, parity = 0;
       // Lane i looks up the page of the i-th box of the next tile to issue, a tile early.
@@ -1038,8 +1038,10 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
       for (bool more = true; more;) {
         issue();
         char* st = ring + stage_out * P::STAGE_BYTES;
-        mbar_wait(&bars[stage_out * 2], parity, a.flags, kWaitSite);
-        __syncwarp();
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars[stage_out * 2], parity, a.flags, kWaitSite))) {
+          again = late = true;
+          break;
+        }
         const uint32_t ok = (uint32_t)bars[stage_out * 2 + 1];
         if (ok != 0xFFFFFFFFu >> (32 - KT)) {
           // what the cache holds behind a sequence's end may be NaN, and 0 * NaN is not 0
@@ -1076,9 +1078,9 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
         }
       }
       if (again) {
-        // the copies under way land first: the joins use the ring's memory
-        while (stage_out != stage_in) {
-          mbar_wait(&bars[stage_out * 2], parity, a.flags, kWaitSite);
+        // the copies under way land first, within another wait each: the joins use the ring's memory
+        for (; late || stage_out != stage_in; late = false) {
+          (void)mbar_wait(&bars[stage_out * 2], parity, a.flags, kWaitSite);
           if (++stage_out == P::STAGES) {
             stage_out = 0;
             parity ^= 1;
