@@ -256,8 +256,8 @@ typedef struct turt_logit_rules {
  * id < vocab (at most 65535 rows); out = logits with equal pitches works in place, other overlaps do
  * not.  A masked entry is -infinity
  * whatever the logit was; a mask without a set bit leaves nothing.  Ids >= vocab, bias ids that do
- * not increase and masks >= n_masks raise TURT_ERR_RANGE at the next synchronization; the ids are
- * skipped, such a mask counts as none. */
+ * not increase and masks >= n_masks raise TURT_ERR_RANGE at the next synchronization; ids >= vocab are
+ * skipped, a row whose bias ids do not increase takes none of its biases, such a mask counts as none. */
 int turt_logit_rules_apply(turt_ctx* ctx, const float* logits, size_t ld, float* out, size_t out_ld, int rows,
                            int vocab, const turt_logit_rules* rules);
 

@@ -128,12 +128,14 @@ __global__ void __launch_bounds__(THREADS, 1536 / THREADS) k_logit_rules(const _
       }
     }
     uint32_t b0 = 0, b1 = 0;
+    bool wild = false;  // bias ids that do not increase
     if (a.r.bias_ids) {
       b0 = a.r.bias_start[r];
       b1 = a.r.bias_start[r + 1];
       for (uint32_t i = b0 + tid; i < b1; i += THREADS) {
         const uint32_t id = a.r.bias_ids[i], e = id - (uint32_t)s0;
-        bad |= id >= (uint32_t)V || (blockIdx.x == 0 && i > b0 && a.r.bias_ids[i - 1] >= id);
+        bad |= id >= (uint32_t)V;
+        wild |= i > b0 && a.r.bias_ids[i - 1] >= id;
         if (e < (uint32_t)SLICE && id < (uint32_t)V) atomicOr(&touched[e >> 5], 1u << (e & 31));
       }
     }
@@ -141,7 +143,13 @@ __global__ void __launch_bounds__(THREADS, 1536 / THREADS) k_logit_rules(const _
     w.rep = a.r.repetition ? a.r.repetition[r] : 1.f;
     w.freq = a.r.frequency ? a.r.frequency[r] : 0.f;
     w.pres = a.r.presence ? a.r.presence[r] : 0.f;
-    __syncthreads();
+    if (__syncthreads_or(wild)) {
+      // an id that comes twice would belong to two threads: the row takes none of its biases
+      bad = true;
+      b1 = b0;
+      for (int e = tid; e < SLICE / 32; e += THREADS) touched[e] = 0;
+      __syncthreads();
+    }
     // ids with a bias (their bits are set already) belong to it, the others to the list
     for (uint32_t i = b0 + tid; i < b1; i += THREADS) {
       const uint32_t id = a.r.bias_ids[i], e = id - (uint32_t)s0;
@@ -384,7 +392,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
 
   bool bad = false;
   int turn = 0;  // slices of rows with ids so far
-  int sorted_row = -1;
+  int sorted_row = -1, checked_row = -1, wild_row = -1;  // wild: its bias ids do not increase
   for (long it = first; it < last; it++) {
     const int k = (int)(it - first), at = k % kRing;
     RuleStage& st = sh.ring[at];
@@ -394,7 +402,7 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
     const int s0 = s.s0, id0 = max(s0, 0), id1 = min(s0 + slice, V);
     if (id1 > id0) {
       float* x = st.x + (VEC ? 0 : (int)skew_of(a.in + (size_t)s.row * a.ld + id0));  // position e = id - s0
-      const uint32_t n_tok = s.i1 - s.i0, n_bias = s.b1 - s.b0, span = id1 - id0;
+      const uint32_t n_tok = s.i1 - s.i0, span = id1 - id0;
       if (n_tok) {
         const uint32_t skew = skew_of(a.r.tokens + s.i0), here = min(n_tok, (uint32_t)kTokenRoom);
         const uint32_t made = s.made > s.i0 ? s.made - s.i0 : 0;
@@ -492,12 +500,24 @@ __global__ void __launch_bounds__(kWorkers + 32, 1)
       }
       const uint32_t* ids = st.bias_ids + skew_of(a.r.bias_ids + s.b0);
       const float* val = st.bias + skew_of(a.r.bias + s.b0);
+      uint32_t n_bias = s.b1 - s.b0;
       const uint32_t n_here = min(n_bias, (uint32_t)kBiasRoom);
       auto bias_id = [&](uint32_t i) { return i < n_here ? ids[i] : a.r.bias_ids[s.b0 + i]; };
+      if (n_bias && s.row != checked_row) {
+        // an id that comes twice would belong to two threads: such a row takes none of its biases
+        checked_row = s.row;
+        bool wild = false;
+        for (uint32_t i = tid + 1; i < n_bias; i += kWorkers) wild |= bias_id(i - 1) >= bias_id(i);
+        if (!workers_all(!wild)) {
+          bad = true;
+          wild_row = s.row;
+        }
+      }
+      if (s.row == wild_row) n_bias = 0;
       // (biases go to the last warps first, ids to the first: few of either keep different warps busy)
       for (uint32_t i = kWorkers - 1 - tid; i < n_bias; i += kWorkers) {
         const uint32_t id = bias_id(i);
-        bad |= id >= (uint32_t)V || (s0 <= 0 && i > 0 && bias_id(i - 1) >= id);
+        bad |= id >= (uint32_t)V;
         if (id - (uint32_t)id0 < span) atomicOr(&sh.cnt[id - (uint32_t)s0], kBiased);
       }
       if (n_tok || n_bias) {
