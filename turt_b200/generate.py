@@ -17,12 +17,13 @@ cache (GpuEngine.pagedAppend / pagedAttention) on the op-by-op GpuGPT.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Callable, Iterable, List, Optional
 
 import numpy as np
 
-from ._lib import CACHE_TYPES, check, lib, u32
+from ._lib import CACHE_TYPES, TurtError, check, lib, u32
 from .pretrain import Mulberry32
 from .runtime import make_logit_rules, make_paged_kv
 
@@ -139,11 +140,29 @@ class LogitRules:
         return self.ctx.download(self._out, self.rows * self.vocab).reshape(self.rows, self.vocab)
 
     def close(self) -> None:
+        """Frees the buffers; their memory comes back with the context's next reclaim()."""
         for b in self._bufs.values():
             b.free()
         if self._out is not None:
             self.ctx.free(self._out)
         self._bufs, self._out = {}, None
+
+
+@contextlib.contextmanager
+def _released(ctx, *things):
+    """Closes `things` on the way out and gives their memory back.  An error that the device reports then does not
+    take the place of the one that led out."""
+    try:
+        yield
+    except BaseException:
+        with contextlib.suppress(TurtError):
+            for t in things:
+                t.close()
+            ctx.reclaim()
+        raise
+    for t in things:
+        t.close()
+    ctx.reclaim()
 
 
 class Generator:
@@ -182,11 +201,12 @@ def generate(model, prompt: Iterable[int], max_new_tokens: int, temperature: flo
     ids = [int(i) for i in prompt]
     n_prompt = len(ids)
     gen = Generator(model)
-    rules = None
+    rules, held = None, contextlib.nullcontext()
     if (repetition_penalty, frequency_penalty, presence_penalty) != (1.0, 0.0, 0.0) or bias or allowed is not None:
         rules = LogitRules(model.ctx, model.cfg.vocab_size, 1, repetition_penalty, frequency_penalty, presence_penalty, bias,
                            allowed)
-    try:
+        held = _released(model.ctx, rules)
+    with held:
         for _ in range(max_new_tokens):
             logits = gen.next_logits(ids)
             if rules is not None:
@@ -196,9 +216,6 @@ def generate(model, prompt: Iterable[int], max_new_tokens: int, temperature: flo
             ids.append(nxt)
             if on_token is not None and on_token(nxt) is False:
                 break
-    finally:
-        if rules is not None:
-            rules.close()
     return ids
 
 
@@ -383,7 +400,7 @@ def generate_batch(gpt, prompts, max_new_tokens: int, temperature: float = 1.0, 
     rules = LogitRules(gpt.engine.ctx, gpt.config["vocabSize"], len(seqs), repetition_penalty, frequency_penalty,
                        presence_penalty, bias, allowed)
     dec = PagedDecoder(gpt, [n + max_new_tokens for n in n_prompt], cache_type, page_size)
-    try:
+    with _released(gpt.engine.ctx, rules, dec):
         logits = dec.prefill(seqs)
         live = [True] * len(seqs)
         for k in range(max_new_tokens):
@@ -399,7 +416,4 @@ def generate_batch(gpt, prompts, max_new_tokens: int, temperature: float = 1.0, 
             if k + 1 == max_new_tokens or not any(live):
                 break
             logits = dec.step([s[-1] if alive else None for s, alive in zip(seqs, live)])
-    finally:
-        rules.close()
-        dec.close()
     return seqs
