@@ -1,0 +1,79 @@
+"""Host side of PagedDecoder without a GPU: an engine that only books its buffers."""
+from types import SimpleNamespace
+
+import pytest
+
+from turt_b200.generate import PagedDecoder
+
+
+class BookedEngine:
+    """Every op is recorded and does nothing; a freed buffer is held until reclaim()."""
+
+    def __init__(self):
+        self.live, self.pending, self.next, self.peak, self.calls, self.uploads = {}, [], 64, 0, [], {}
+        self.ctx = SimpleNamespace(upload=self._upload)
+
+    def _upload(self, p, a):
+        self.uploads[p] = a.copy()
+
+    def buffer(self, elems):
+        p, self.next = self.next, self.next + (1 << 40)
+        self.live[p] = elems
+        self.peak = max(self.peak, sum(self.live.values()))
+        return p
+
+    def indexBuffer(self, a):
+        p = self.buffer(a.size)
+        self._upload(p, a)
+        return p
+
+    def free(self, p):
+        self.pending.append(p)
+
+    def reclaim(self):
+        for p in self.pending:
+            del self.live[p]
+        self.pending = []
+
+    def pagedAttentionWorkspace(self, kv, heads):
+        return 4096
+
+    def __getattr__(self, name):
+        return lambda *a, **kw: self.calls.append((name, a, kw))
+
+
+def booked_gpt(layers, arch="modern", E=8, H=2, block=256):
+    t = lambda: SimpleNamespace(buffer=1)  # noqa: E731
+    names = ("ln1g", "ln1b", "qW", "qb", "kW", "kb", "vW", "vb", "projW", "projb", "ln2g", "ln2b", "gateW", "upW", "downW", "fcW",
+             "fcb", "mpW", "mpb")
+    return SimpleNamespace(fused=False, engine=BookedEngine(), modern=arch == "modern", hidden=4 * E, headScale=0.5, wte=t(),
+                           wpe=None if arch == "modern" else t(), lnfg=t(), lnfb=t(), blocks=[{n: t() for n in names}] * layers,
+                           config=dict(nEmbd=E, nHead=H, vocabSize=11, nLayer=layers, blockSize=block))
+
+
+def prefill_peak(layers, prompts, arch="modern"):
+    g = booked_gpt(layers, arch)
+    dec = PagedDecoder(g, [len(p) + 4 for p in prompts])
+    held = sum(g.engine.live.values())
+    dec.prefill(prompts)
+    assert sum(g.engine.live.values()) == held  # a forward leaves nothing behind
+    dec.step([1] * len(prompts))
+    assert sum(g.engine.live.values()) == held
+    peak = g.engine.peak - held
+    dec.close()
+    assert not g.engine.live
+    return peak
+
+
+@pytest.mark.parametrize("arch", ["modern", "gpt2"])
+def test_prefill_memory_does_not_grow_with_the_layers(arch):
+    prompts = [[1] * 200, [2] * 7, [3] * 90]
+    assert prefill_peak(12, prompts, arch) == prefill_peak(1, prompts, arch)
+
+
+def test_prefill_memory_of_many_prompts():
+    """One matrix of scores serves all prompts: what else there is grows with the rows (16 values of width E or hidden a
+    row, at most, and a few indices)."""
+    one, many = prefill_peak(2, [[1] * 200]), prefill_peak(2, [[1] * 200] * 16)
+    assert one >= 2 * 200 * 200
+    assert many - one <= 15 * 200 * 16 * 4 * 8 and many < one + 2 * 200 * 200 * 15 / 2

@@ -252,50 +252,53 @@ class PagedDecoder:
         self.work = self.e.pagedAttentionWorkspace(self.kv[0], self.H)
         self.space = self.e.buffer((self.work + 3) // 4)
         self.logits = self.e.buffer(self.batch * self.V)
-        self.tmp = []
+        self.tmp, self.indices = {}, []
 
-    def _new(self, n: int) -> int:
-        self.tmp.append(self.e.buffer(n))
-        return self.tmp[-1]
+    def _new(self, name: str, n: int) -> int:
+        """The forward's buffer `name`.  All layers and prompts use the same one after another, which the stream orders;
+        the first use takes the largest size."""
+        if name not in self.tmp:
+            self.tmp[name] = self.e.buffer(n)
+        return self.tmp[name]
 
     def _index(self, a) -> int:
-        self.tmp.append(self.e.indexBuffer(a))
-        return self.tmp[-1]
+        self.indices.append(self.e.indexBuffer(a))
+        return self.indices[-1]
 
-    def _lin(self, x, w, rows, k, n, bias=None) -> int:
-        out = self._new(rows * n)
+    def _lin(self, name, x, w, rows, k, n, bias=None) -> int:
+        out = self._new(name, rows * n)
         self.e.matmulInto(x, w.buffer, out, rows, k, n, 1, False, False, False)
         if bias is not None:
             self.e.ewise(out, bias.buffer, out, rows * n, n, 0, False)
         return out
 
     def _norm(self, x, rows, g, b) -> int:
-        out, stat = self._new(rows * self.E), self._new(2 * rows)
+        out, stat = self._new("norm", rows * self.E), self._new("stat", 2 * rows)
         if self.gpt.modern:
             self.e.rmsFwd(x, g.buffer, out, stat, rows, self.E, 1e-5)
         else:
             self.e.lnFwd(x, g.buffer, b.buffer, out, stat, stat + 4 * rows, rows, self.E, 1e-5)
         return out
 
-    def _add(self, a, b, n) -> int:
-        out = self._new(n)
+    def _add(self, name, a, b, n) -> int:
+        out = self._new(name, n)
         self.e.ewise(a, b, out, n, n, 0, False)
         return out
 
-    def _prompt_attention(self, q, k, v, out, t) -> None:
+    def _prompt_attention(self, q, k, v, out, t, longest) -> None:
         """Causal attention inside one prompt of t rows (q rotated already), with the ops of the tape."""
         e, H, hd, n = self.e, self.H, self.hd, t * self.E
 
-        def heads(x):
-            y = self._new(n)
+        def heads(name, x):
+            y = self._new(name, longest * self.E)
             e.permute4(x, y, [1, t, H, hd], [0, 2, 1, 3], n, False)
             return y
-        qh, kh, vh = heads(q), heads(k), heads(v)
+        qh, kh, vh = heads("qh", q), heads("kh", k), heads("vh", v)
         if self.gpt.modern:
-            r = self._new(n)
+            r = self._new("kr", longest * self.E)
             e.ropeInto(kh, r, H, t, hd, 10000.0)
             kh = r
-        s, y = self._new(H * t * t), self._new(n)
+        s, y = self._new("scores", H * longest * longest), self._new("yh", longest * self.E)
         e.matmulInto(qh, kh, s, t, hd, t, H, False, True, False)
         e.scale(s, s, H * t * t, self.gpt.headScale, False)
         e.maskInto(s, s, H, t)
@@ -309,49 +312,53 @@ class PagedDecoder:
         e, g, E, rows = self.e, self.gpt, self.E, len(ids)
         e.ctx.upload(self.d_lens, u32(self.lens))
         d_start = None if start is None else self._index(start)
-        x = self._new(rows * E)
+        x = self._new("x", rows * E)
         e.gatherInto(g.wte.buffer, self._index(ids), x, rows, E, self.V)
         if g.wpe is not None:
-            p = self._new(rows * E)
+            p = self._new("out", rows * E)
             e.gatherInto(g.wpe.buffer, self._index(pos), p, rows, E, g.config["blockSize"])
-            x = self._add(x, p, rows * E)
+            self._add("x", x, p, rows * E)
         for blk, kv in zip(g.blocks, self.kv):
             y = self._norm(x, rows, blk["ln1g"], blk.get("ln1b"))
-            q, k, v = (self._lin(y, blk[n + "W"], rows, E, E, blk.get(n + "b")) for n in "qkv")
-            qr, att = self._new(rows * E), self._new(rows * E)
+            q, k, v = (self._lin(n, y, blk[n + "W"], rows, E, E, blk.get(n + "b")) for n in "qkv")
+            qr, att = self._new("qr", rows * E), self._new("att", rows * E)
             e.pagedAppend(kv, k, E, v, E, rows, start=d_start, q=q, qStride=E, qOut=qr, qOutStride=E, nHead=self.H,
                           rotDim=self.hd if g.modern else 0)
             if start is None:
                 e.pagedAttention(kv, qr, E, att, E, self.H, self.space, self.work, scale=g.headScale)
             else:
+                longest = int(np.diff(start).max())
                 for lo, hi in zip(start[:-1], start[1:]):
                     at = 4 * int(lo) * E
-                    self._prompt_attention(qr + at, k + at, v + at, att + at, int(hi - lo))
-            h = self._add(x, self._lin(att, blk["projW"], rows, E, E, blk.get("projb")), rows * E)
+                    self._prompt_attention(qr + at, k + at, v + at, att + at, int(hi - lo), longest)
+            h = self._add("h", x, self._lin("out", att, blk["projW"], rows, E, E, blk.get("projb")), rows * E)
             y = self._norm(h, rows, blk["ln2g"], blk.get("ln2b"))
             n = g.hidden
             if g.modern:
-                a, u = self._lin(y, blk["gateW"], rows, E, n), self._lin(y, blk["upW"], rows, E, n)
-                act = self._new(rows * n)
+                a, u = self._lin("gate", y, blk["gateW"], rows, E, n), self._lin("up", y, blk["upW"], rows, E, n)
+                act = self._new("act", rows * n)
                 e.siluInto(a, act, rows * n)
                 e.ewise(act, u, act, rows * n, rows * n, 2, False)
-                m = self._lin(act, blk["downW"], rows, n, E)
+                m = self._lin("out", act, blk["downW"], rows, n, E)
             else:
-                f = self._lin(y, blk["fcW"], rows, E, n, blk["fcb"])
-                act = self._new(rows * n)
+                f = self._lin("gate", y, blk["fcW"], rows, E, n, blk["fcb"])
+                act = self._new("act", rows * n)
                 e.geluInto(f, act, rows * n)
-                m = self._lin(act, blk["mpW"], rows, n, E, blk["mpb"])
-            x = self._add(h, m, rows * E)
+                m = self._lin("out", act, blk["mpW"], rows, n, E, blk["mpb"])
+            self._add("x", h, m, rows * E)
         if start is not None:
-            last = self._new(self.batch * E)
+            last = self._new("h", self.batch * E)
             e.gatherInto(x, self._index(start[1:] - 1), last, self.batch, E, rows)
             x = last
         y = self._norm(x, self.batch, g.lnfg, g.lnfb)
         e.matmulInto(y, g.wte.buffer, self.logits, self.batch, E, self.V, 1, False, True, False)
-        for b in self.tmp:
-            e.free(b)
-        self.tmp = []
+        self._drop()
         e.reclaim()
+
+    def _drop(self) -> None:
+        for b in (*self.tmp.values(), *self.indices):
+            self.e.free(b)
+        self.tmp, self.indices = {}, []
 
     def prefill(self, prompts) -> int:
         self.lens = np.array([len(p) for p in prompts])
@@ -372,9 +379,10 @@ class PagedDecoder:
         for kv in self.kv:
             self.e.free(kv.k)
             self.e.free(kv.v)
-        for b in (self.table, self.d_lens, self.space, self.logits, *self.tmp):
+        for b in (self.table, self.d_lens, self.space, self.logits):
             self.e.free(b)
-        self.kv, self.tmp = [], []
+        self._drop()
+        self.kv = []
         self.e.reclaim()
 
 
