@@ -77,3 +77,20 @@ def test_prefill_memory_of_many_prompts():
     one, many = prefill_peak(2, [[1] * 200]), prefill_peak(2, [[1] * 200] * 16)
     assert one >= 2 * 200 * 200
     assert many - one <= 15 * 200 * 16 * 4 * 8 and many < one + 2 * 200 * 200 * 15 / 2
+
+
+def test_a_forward_that_fails_keeps_no_buffer():
+    """The next forward asks for its own sizes."""
+    g = booked_gpt(2)
+    dec = PagedDecoder(g, [40, 40])
+    held = set(g.engine.live)
+    g.engine.pagedAttention = lambda *a, **kw: 1 // 0
+    dec.prefill([[1] * 3, [2]])
+    with pytest.raises(ZeroDivisionError):
+        dec.step([1, 1])
+    g.engine.pagedAttention = lambda *a, **kw: None
+    g.engine.reclaim()
+    assert set(g.engine.live) == held
+    g.engine.peak = 0
+    dec.prefill([[1] * 30, [2] * 20])
+    assert g.engine.peak - sum(g.engine.live.values()) >= 2 * 30 * 30  # scores of 30 rows

@@ -309,6 +309,13 @@ class PagedDecoder:
     def _forward(self, ids, pos, start) -> None:
         """One forward of rows (ids at positions pos): the prompts one after another (start: where each
         begins) or, start None, one new token per sequence."""
+        try:
+            self._run(ids, pos, start)
+        finally:
+            self._drop()  # the next forward's sizes are others
+        self.e.reclaim()
+
+    def _run(self, ids, pos, start) -> None:
         e, g, E, rows = self.e, self.gpt, self.E, len(ids)
         e.ctx.upload(self.d_lens, u32(self.lens))
         d_start = None if start is None else self._index(start)
@@ -352,8 +359,6 @@ class PagedDecoder:
             x = last
         y = self._norm(x, self.batch, g.lnfg, g.lnfb)
         e.matmulInto(y, g.wte.buffer, self.logits, self.batch, E, self.V, 1, False, True, False)
-        self._drop()
-        e.reclaim()
 
     def _drop(self) -> None:
         for b in (*self.tmp.values(), *self.indices):
