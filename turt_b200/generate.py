@@ -237,7 +237,8 @@ class PagedDecoder:
             raise ValueError(f"{max(lengths)} positions exceed block size {c['blockSize']}")
         need = [-(-n // page_size) for n in lengths]
         self.n_pages, self.width = sum(need), max(need)
-        table = np.zeros((self.batch, self.width), np.uint32)
+        self.room = np.array(lengths, np.int64)
+        table = np.full((self.batch, self.width), 0xFFFFFFFF, np.uint32)  # no page
         page = 0
         for b, n in enumerate(need):
             table[b, :n] = np.arange(page, page + n)
@@ -365,19 +366,30 @@ class PagedDecoder:
             self.e.free(b)
         self.tmp, self.indices = {}, []
 
+    def _fits(self, lens) -> None:
+        for i in np.flatnonzero(lens > self.room):
+            raise ValueError(f"sequence {i} would hold {lens[i]} positions, {self.room[i]} are reserved")
+
     def prefill(self, prompts) -> int:
-        self.lens = np.array([len(p) for p in prompts])
+        if len(prompts) != self.batch or not all(len(p) for p in prompts):
+            raise ValueError(f"expected {self.batch} prompts of one token or more")
+        lens = np.array([len(p) for p in prompts])
+        self._fits(lens)
+        self.lens = lens
         ids = np.concatenate([np.asarray(p) for p in prompts])
-        self._forward(u32(ids), u32(np.concatenate([np.arange(n) for n in self.lens])),
-                      np.concatenate(([0], np.cumsum(self.lens))))
+        self._forward(u32(ids), u32(np.concatenate([np.arange(n) for n in lens])), np.concatenate(([0], np.cumsum(lens))))
         return self.logits
 
     def step(self, tokens) -> int:
         """One token per sequence; None leaves a sequence idle (its logits are then meaningless)."""
+        if len(tokens) != self.batch:
+            raise ValueError(f"expected {self.batch} tokens, got {len(tokens)}")
         live = np.array([t is not None for t in tokens])
-        held, self.lens = self.lens, np.where(live, self.lens + 1, 0)
-        self._forward(u32([0 if t is None else t for t in tokens]), u32(np.maximum(self.lens - 1, 0)), None)
-        self.lens = np.where(live, self.lens, held)
+        lens = np.where(live, self.lens + 1, 0)
+        self._fits(lens)
+        held, self.lens = self.lens, lens
+        self._forward(u32([0 if t is None else t for t in tokens]), u32(np.maximum(lens - 1, 0)), None)
+        self.lens = np.where(live, lens, held)
         return self.logits
 
     def close(self) -> None:
