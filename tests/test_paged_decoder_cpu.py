@@ -119,3 +119,13 @@ def test_no_position_beyond_what_is_reserved():
     assert len(g.engine.calls) == n and dec.lens.tolist() == [18, 2]
     dec.step([None, 1])
     assert dec.lens.tolist() == [18, 3]
+
+
+def test_a_step_that_fails_leaves_the_lengths():
+    g = booked_gpt(1)
+    dec = PagedDecoder(g, [18, 40])
+    dec.prefill([[1] * 3, [2]])
+    g.engine.pagedAttention = lambda *a, **kw: 1 // 0
+    with pytest.raises(ZeroDivisionError):
+        dec.step([None, 1])
+    assert dec.lens.tolist() == [3, 1]

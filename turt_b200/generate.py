@@ -377,7 +377,11 @@ class PagedDecoder:
         self._fits(lens)
         self.lens = lens
         ids = np.concatenate([np.asarray(p) for p in prompts])
-        self._forward(u32(ids), u32(np.concatenate([np.arange(n) for n in lens])), np.concatenate(([0], np.cumsum(lens))))
+        try:
+            self._forward(u32(ids), u32(np.concatenate([np.arange(n) for n in lens])), np.concatenate(([0], np.cumsum(lens))))
+        except BaseException:
+            self.lens = np.zeros(self.batch, np.int64)  # what the pages hold is not known
+            raise
         return self.logits
 
     def step(self, tokens) -> int:
@@ -388,8 +392,11 @@ class PagedDecoder:
         lens = np.where(live, self.lens + 1, 0)
         self._fits(lens)
         held, self.lens = self.lens, lens
-        self._forward(u32([0 if t is None else t for t in tokens]), u32(np.maximum(lens - 1, 0)), None)
-        self.lens = np.where(live, lens, held)
+        try:
+            self._forward(u32([0 if t is None else t for t in tokens]), u32(np.maximum(lens - 1, 0)), None)
+            held = np.where(live, lens, held)
+        finally:
+            self.lens = held
         return self.logits
 
     def close(self) -> None:
