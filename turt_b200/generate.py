@@ -102,9 +102,10 @@ class LogitRules:
     def _put(self, name: str, a: np.ndarray) -> int:
         return self._bufs.setdefault(name, _Grown(self.ctx)).put(a)
 
-    def apply(self, d_logits: int, prompts, generated) -> np.ndarray:
+    def apply(self, d_logits: int, prompts, generated, live=None) -> np.ndarray:
         """The logits [rows][vocab] at d_logits under the rules, on the host; prompts and generated hold
-        each row's ids."""
+        each row's ids.  Rows that live (a truth value per row, default all) leaves out get no mask: allowed is
+        not asked about them."""
         kw = {}
         if self.penalties:
             lens = np.array([[len(p), len(g)] for p, g in zip(prompts, generated)], np.int64)
@@ -120,7 +121,8 @@ class LogitRules:
                       bias=self._put("bias", np.array([v for p in pairs for _, v in p], np.float32)),
                       bias_start=self._put("bias_start", u32(np.concatenate(([0], np.cumsum([len(p) for p in pairs]))))))
         if self.allowed is not None:
-            masks = [self.allowed(r, [*prompts[r], *generated[r]]) for r in range(self.rows)]
+            masks = [self.allowed(r, [*prompts[r], *generated[r]]) if live is None or live[r] else None
+                     for r in range(self.rows)]
             some = [np.asarray(m, bool) for m in masks if m is not None]
             for m in some:
                 if m.shape != (self.vocab,):
@@ -437,7 +439,8 @@ def generate_batch(gpt, prompts, max_new_tokens: int, temperature: float = 1.0, 
         live = [True] * len(seqs)
         for k in range(max_new_tokens):
             if rules.active:
-                rows = rules.apply(logits, [s[:n] for s, n in zip(seqs, n_prompt)], [s[n:] for s, n in zip(seqs, n_prompt)])
+                rows = rules.apply(logits, [s[:n] for s, n in zip(seqs, n_prompt)], [s[n:] for s, n in zip(seqs, n_prompt)],
+                                   live)
             else:
                 rows = gpt.engine.read(logits, len(seqs) * dec.V).reshape(len(seqs), dec.V)
             for i, s in enumerate(seqs):
