@@ -19,7 +19,6 @@ class Context:
         self._h = C.c_void_p()
         check(lib().turt_init(device, C.byref(self._h)))
         self.device = device
-        self._stream = lib().turt_ctx_stream(self._h) or 0
 
     @property
     def handle(self):
@@ -30,7 +29,6 @@ class Context:
 
     def set_stream(self, stream_ptr: int) -> None:
         check(lib().turt_ctx_set_stream(self._h, stream_ptr))
-        self._stream = stream_ptr or 0
 
     def set_precision(self, precision: int) -> None:
         """0 = fp32 CUDA cores (op level only), 1 = plain TF32, 3 = error-compensated 3xTF32 (default)."""
@@ -44,7 +42,7 @@ class Context:
 
     @property
     def stream(self) -> int:
-        return self._stream
+        return lib().turt_ctx_stream(self._h) or 0
 
     # device buffers (raw pointers)
     def buffer(self, elems: int) -> int:
