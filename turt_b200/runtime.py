@@ -19,6 +19,7 @@ class Context:
         self._h = C.c_void_p()
         check(lib().turt_init(device, C.byref(self._h)))
         self.device = device
+        self._stream_of = lib().turt_ctx_stream  # asked for before every call of some programs
 
     @property
     def handle(self):
@@ -42,7 +43,7 @@ class Context:
 
     @property
     def stream(self) -> int:
-        return lib().turt_ctx_stream(self._h) or 0
+        return self._stream_of(self._h) or 0
 
     # device buffers (raw pointers)
     def buffer(self, elems: int) -> int:
