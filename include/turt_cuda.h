@@ -361,7 +361,8 @@ int turt_forward_device(turt_model* model, const uint32_t* ids, const uint32_t* 
 int turt_generate_prefill(turt_model* model, const uint32_t* ids, int t, float* logits_out);
 int turt_generate_step(turt_model* model, uint32_t id, int pos, float* logits_out);
 /* Device pointer of the logits (vocab_size floats) that the last prefill or step wrote, for rules on
- * them (turt_logit_rules_apply); valid until the model's next call. */
+ * them (turt_logit_rules_apply); valid until the model's next call.  TURT_ERR_INVALID where another forward has
+ * taken their place since. */
 int turt_generate_logits(turt_model* model, const float** d_logits);
 /* clipGradNorm (src/optim/clip.ts:7-24) over all gradients; norm_out may be NULL. */
 int turt_clip_grad_norm(turt_model* model, double max_norm, double* norm_out);

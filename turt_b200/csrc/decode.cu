@@ -466,7 +466,7 @@ extern "C" int turt_generate_step(turt_model* m, uint32_t id, int pos, float* lo
 
 extern "C" int turt_generate_logits(turt_model* m, const float** d_logits) {
   TURT_REQUIRE(m && d_logits, "generate_logits: null argument");
-  TURT_REQUIRE(m->kcache && m->dec_logits, "generate_logits: nothing generated yet");
+  TURT_REQUIRE(m->kcache && m->dec_logits, "generate_logits: nothing generated yet, or another forward has run since");
   *d_logits = m->dec_logits;
   return OK;
 }

@@ -135,6 +135,7 @@ void build_layout(turt_model* m) {
 void free_workspace(turt_model* m) {
   if (m->ws) cudaFree(m->ws);
   m->ws = nullptr;
+  m->dec_logits = nullptr;
   m->capN = 0;
   m->capS = 0;
   m->act.clear();
@@ -301,6 +302,7 @@ int forward(turt_model* m, int B, int T, bool train, float loss_scale, bool logi
   int* flags = m->ctx->flags;
   const int N = B * T, E = m->cfg.n_embd, H = m->cfg.n_head, hd = E / H, V = m->cfg.vocab_size, h = m->hid;
   const float* P = m->P;
+  m->dec_logits = nullptr;  // m->logits is written anew
   RC(embed_fwd(st, P + m->wte, m->modern ? nullptr : P + m->wpe, m->d_ids, m->act.empty() ? m->xL : m->act[0].x, N, T,
                E, V, flags));
   for (int l = 0; l < m->cfg.n_layer; l++) {

@@ -81,7 +81,7 @@ struct turt_model {
   float *kcache = nullptr, *vcache = nullptr, *dec = nullptr;
   size_t dec_floats = 0;
   int dec_len = 0;
-  const float* dec_logits = nullptr;  // logits of the last prefill or step (device)
+  const float* dec_logits = nullptr;  // logits of the last prefill or step (device), null after another forward
   // The decode step is captured once into a CUDA graph that reads (token, position) from a
   // device cell; each step copies the pair there from pinned memory and replays the graph.
   int* dec_tok = nullptr;
