@@ -42,3 +42,14 @@ def test_stopped_sequences_are_left_alone(rules):
     assert [len(s) for s in out] == [3, 6, 7] and made == [2, 4, 6]
     assert [asked.count(i) for i in range(3)] == made
     assert [r.n_masks for r in rules] == [3, 3, 2, 2, 1, 1]
+
+
+def test_rules_refuse_another_number_of_rows(rules):
+    """The device reads an entry per row of every array."""
+    r = gen.LogitRules(DeferredContext(), 11, 3, frequency=0.5)
+    for args in (([[1]] * 2, [[]] * 2), ([[1]] * 3, [[]] * 2), ([[1]] * 4, [[]] * 3), ([[1]] * 3, [[]] * 3, [True] * 2)):
+        with pytest.raises(ValueError, match="expected 3 rows"):
+            r.apply(64, *args)
+    assert not rules and not r.ctx.live
+    r.apply(64, [[1]] * 3, [[]] * 3, [True, False, True])
+    assert len(rules) == 1

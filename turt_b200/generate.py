@@ -106,6 +106,9 @@ class LogitRules:
         """The logits [rows][vocab] at d_logits under the rules, on the host; prompts and generated hold
         each row's ids.  Rows that live (a truth value per row, default all) leaves out get no mask: allowed is
         not asked about them."""
+        for what in (prompts, generated) if live is None else (prompts, generated, live):
+            if len(what) != self.rows:
+                raise ValueError(f"expected {self.rows} rows, got {len(what)}")
         kw = {}
         if self.penalties:
             lens = np.array([[len(p), len(g)] for p, g in zip(prompts, generated)], np.int64)
