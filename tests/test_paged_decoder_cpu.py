@@ -3,6 +3,7 @@ from types import SimpleNamespace
 
 import pytest
 
+from turt_b200._lib import ERR_CUDA, TurtError
 from turt_b200.generate import PagedDecoder
 
 
@@ -129,3 +130,32 @@ def test_a_step_that_fails_leaves_the_lengths():
     with pytest.raises(ZeroDivisionError):
         dec.step([None, 1])
     assert dec.lens.tolist() == [3, 1]
+
+
+@pytest.mark.parametrize("after", range(9))
+def test_a_reservation_that_fails_keeps_nothing(after):
+    """Memory that runs out at any of the buffers: those taken before it are given back, and a smaller batch fits."""
+    g = booked_gpt(3)
+    e, left = g.engine, [after]
+    take = e.buffer
+
+    def buffer(n):
+        if left[0] == 0:
+            raise TurtError(ERR_CUDA, "out of memory")
+        left[0] -= 1
+        return take(n)
+    e.buffer = buffer
+    with pytest.raises(TurtError, match="out of memory"):
+        PagedDecoder(g, [18, 40])
+    assert not e.live
+    left[0] = 100
+    PagedDecoder(g, [18]).close()
+    assert not e.live
+
+
+def test_closing_twice_frees_once():
+    g = booked_gpt(1)
+    dec = PagedDecoder(g, [18])
+    dec.close()
+    dec.close()
+    assert not g.engine.live

@@ -248,17 +248,28 @@ class PagedDecoder:
         for b, n in enumerate(need):
             table[b, :n] = np.arange(page, page + n)
             page += n
-        self.table = self.e.indexBuffer(table)
-        self.d_lens = self.e.indexBuffer(np.zeros(self.batch, np.uint32))
         self.lens = np.zeros(self.batch, np.int64)
+        self.held, self.tmp, self.indices = [], {}, []
+        try:
+            self._reserve(table, cache_type, page_size)
+        except BaseException:
+            with contextlib.suppress(TurtError):
+                self.close()
+            raise
+
+    def _reserve(self, table, cache_type, page_size) -> None:
+        def keep(p):
+            self.held.append(p)
+            return p
+        self.table = keep(self.e.indexBuffer(table))
+        self.d_lens = keep(self.e.indexBuffer(np.zeros(self.batch, np.uint32)))
         per = self.n_pages * page_size * self.E
         words = per if cache_type == "f32" else (per + 1) // 2
-        self.kv = [make_paged_kv(self.e.buffer(words), self.e.buffer(words), self.table, self.d_lens, cache_type,
+        self.kv = [make_paged_kv(keep(self.e.buffer(words)), keep(self.e.buffer(words)), self.table, self.d_lens, cache_type,
                                  self.n_pages, page_size, self.H, self.hd, self.batch, self.width) for _ in range(self.L)]
         self.work = self.e.pagedAttentionWorkspace(self.kv[0], self.H)
-        self.space = self.e.buffer((self.work + 3) // 4)
-        self.logits = self.e.buffer(self.batch * self.V)
-        self.tmp, self.indices = {}, []
+        self.space = keep(self.e.buffer((self.work + 3) // 4))
+        self.logits = keep(self.e.buffer(self.batch * self.V))
 
     def _new(self, name: str, n: int) -> int:
         """The forward's buffer `name`.  All layers and prompts use the same one after another, which the stream orders;
@@ -405,13 +416,10 @@ class PagedDecoder:
         return self.logits
 
     def close(self) -> None:
-        for kv in self.kv:
-            self.e.free(kv.k)
-            self.e.free(kv.v)
-        for b in (self.table, self.d_lens, self.space, self.logits):
+        for b in self.held:
             self.e.free(b)
+        self.held = []
         self._drop()
-        self.kv = []
         self.e.reclaim()
 
 
