@@ -121,3 +121,24 @@ def test_values_near_the_largest(eng, dtype, dim, heads, size):
     want, wl, tol, ltol = expect(c, q, heads)
     close(out, want, tol)
     close(lse, wl, ltol)
+
+
+@pytest.mark.parametrize("dtype,dim,heads", NARROW_AND_WIDE)
+@pytest.mark.parametrize("window", [0, 70])
+def test_sequences_that_are_not_finite_among_others(eng, dtype, dim, heads, window):
+    """NaN in some sequences of a ragged batch, several of them in a warp's stretch: the others do not notice."""
+    lens = [(i * 37) % 120 for i in range(150)] + [900, 2500, 0, 1]
+    c = Cache(lens, 1, dim, 16, dtype, seed=dim)
+    bad = [b for b, n in enumerate(lens) if n and b % 7 == 3]
+    for b in bad:
+        pages, slots = c._at(b, lens[b])
+        c.view(c.v if b % 2 else c.k)[pages[-1], slots[-1], :, 1] = math.nan
+    q = torch.randn(len(lens), heads * dim, generator=torch.Generator().manual_seed(dim)).cuda()
+    out, lse = attend(eng, c, q, heads, window=window)
+    want, wl, tol, ltol = expect(c, q, heads, window=window)
+    good = [b for b in range(len(lens)) if b not in bad]
+    close(out[good], want[good], tol[good])
+    close(lse[good], wl[good], ltol[good])
+    assert torch.isnan(out.view(len(lens), heads, dim)[bad][..., 1]).all()
+    again, _ = attend(eng, c, q, heads, window=window)
+    assert torch.equal(again[good], out[good])
