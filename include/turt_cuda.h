@@ -50,6 +50,9 @@ int turt_ctx_destroy(turt_ctx* ctx);
 /* Run all of this context's work on an external CUDA stream (cudaStream_t as void*). */
 int turt_ctx_set_stream(turt_ctx* ctx, void* stream);
 void* turt_ctx_stream(turt_ctx* ctx);
+/* Address of the context's stream (a cudaStream_t), for hosts that look before every call: what it holds is what
+ * turt_ctx_stream gives, until turt_ctx_destroy.  NULL for a null context. */
+void* turt_ctx_stream_cell(turt_ctx* ctx);
 /* Waits for the context's stream and reports device-side error flags (range, timeout). */
 int turt_synchronize(turt_ctx* ctx);
 /* Self-test of the bounded device wait that every tcgen05 kernel of this library uses: one

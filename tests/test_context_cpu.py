@@ -5,25 +5,27 @@ import turt_b200.runtime as rt
 
 
 class FakeLibrary:
-    """Contexts as entries of a dict, the stream of each in it."""
+    """One context, its stream in a cell of its own."""
 
     def __init__(self):
-        self.streams = {}
+        self.cell, self.gone = C.c_void_p(), False
 
     def turt_init(self, device, out):
         out._obj.value = 4096
-        self.streams[4096] = 77
+        self.cell.value = 77
         return 0
 
-    def turt_ctx_stream(self, h):
-        return self.streams.get(h.value)
+    def turt_ctx_stream_cell(self, h):
+        assert h.value == 4096 and not self.gone
+        return C.addressof(self.cell)
 
     def turt_ctx_set_stream(self, h, stream):
-        self.streams[h.value] = stream
+        self.cell.value = stream
         return 0
 
     def turt_ctx_destroy(self, h):
-        del self.streams[h.value]
+        self.gone = True
+        self.cell.value = 13  # the memory belongs to someone else now
         return 0
 
 
@@ -44,3 +46,4 @@ def test_stream_is_the_librarys(monkeypatch):
 
 def test_stream_of_no_context():
     assert not rt.lib().turt_ctx_stream(C.c_void_p())
+    assert not rt.lib().turt_ctx_stream_cell(C.c_void_p())

@@ -131,6 +131,7 @@ int turt_ctx_set_stream(turt_ctx* ctx, void* stream) {
   return OK;
 }
 
+void* turt_ctx_stream_cell(turt_ctx* ctx) { return ctx ? &ctx->stream : nullptr; }
 void* turt_ctx_stream(turt_ctx* ctx) { return ctx ? reinterpret_cast<void*>(ctx->stream) : nullptr; }
 
 int turt_set_precision(turt_ctx* ctx, int precision) {

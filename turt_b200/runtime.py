@@ -18,8 +18,8 @@ class Context:
     def __init__(self, device: int = 0):
         self._h = C.c_void_p()
         check(lib().turt_init(device, C.byref(self._h)))
+        self._stream = C.c_void_p.from_address(lib().turt_ctx_stream_cell(self._h))
         self.device = device
-        self._stream_of = lib().turt_ctx_stream  # asked for before every call of some programs
 
     @property
     def handle(self):
@@ -43,7 +43,7 @@ class Context:
 
     @property
     def stream(self) -> int:
-        return self._stream_of(self._h) or 0
+        return self._stream.value or 0
 
     # device buffers (raw pointers)
     def buffer(self, elems: int) -> int:
@@ -74,6 +74,7 @@ class Context:
 
     def close(self) -> None:
         if self._h:
+            self._stream = C.c_void_p()
             lib().turt_ctx_destroy(self._h)
             self._h = C.c_void_p()
 
