@@ -2,18 +2,18 @@
 //
 //   s_j = scale q . k_j,  out = sum_j 2^(s_j' - m) v_j / sum_j 2^(s_j' - m),  s' = s log2(e)
 //
-// Every cached key and value is read once and used by the heads of its group only, so the bound is
-// the memory bandwidth.  The positions of all sequences and key heads form one line of tiles, cut
-// into equal stretches, one per warp of a grid that fills the GPU once: ragged lengths, one long
-// sequence and many short ones load all warps alike, whatever the lengths are (they are read on the
-// device).  A warp streams its tiles through a ring of shared memory of its own, filled by bulk tensor
-// copies that one lane issues, so nothing but its own copies holds it up; it runs the online softmax
-// of its stretch in registers.  A part of a sequence that a warp did not see whole is joined with its
-// neighbours': first inside the block, then by the last block to arrive, always in the order of
-// positions.
+// Every cached key and value is used by the heads of its group only and read once for eight of them
+// (for four where heads have more than 128 elements), so the bound is the memory bandwidth.  The
+// positions of all sequences and key heads form one line of tiles, cut into equal stretches, one per
+// warp of a grid that fills the GPU once: ragged lengths, one long sequence and many short ones load
+// all warps alike, whatever the lengths are (they are read on the device).  A warp streams its tiles
+// through a ring of shared memory of its own, filled by bulk tensor copies that one lane issues, so
+// nothing but its own copies holds it up; it runs the online softmax of its stretch in registers.  A
+// part of a sequence that a warp did not see whole is joined with its neighbours': first inside the
+// block, then by the last block to arrive, always in the order of positions.
 //
 // Measured on a B200 (changing inputs): 96 sequences of up to 8192, 32 query / 8 key heads of 128, bf16
-// (1.63 GB): 281 us, 5.8 TB/s; one of 131001 (537 MB): 98 us, 5.5 TB/s; 64 of up to 1024, 12 heads of
+// (1.63 GB): 260 us, 6.3 TB/s; one of 131001 (537 MB): 93 us, 5.7 TB/s; 64 of up to 1024, 12 heads of
 // 64, fp32 (204 MB): 41 us, 5.0 TB/s.  Of the last, about 5 us pass before the first tile has arrived
 // (length -> page table -> copy, each a trip to memory) and 4 us in the joins.
 #include <math.h>
@@ -385,7 +385,7 @@ struct PathMma {
   using Type = T;
   using H = Half2<T>;
   // heads of up to 64 elements: twice the positions, for the work per tile that does not grow with them
-  // (16 / 8 heads of 64, 32 x 4000 positions: 50 us, with tiles of 16 positions 66 us)
+  // (16 / 8 heads of 64, 32 x 4000 positions: 49 us; with tiles of 16 positions it was 66, and 50)
   static constexpr int KT = KD <= 4 ? 32 : 16, WARPS = 8, NB = KT / 8;
   static constexpr int MAX_DIM = KD * 16;
   static constexpr bool RING = true;
@@ -1260,9 +1260,9 @@ int attend_launch(turt_ctx* ctx, AttendArgs a, int part) {
   static std::atomic<uint64_t> done{0};
   a.part = part;
   a.chunks = (a.group + part - 1) / part;
-  // At least 32 positions per warp (1 x 1000 positions, 6 fp32 heads of 64: 10.1 us, with 64 at least 13.4);
-  // whole parts in a block where the longest has up to 64 per warp (1 x 200: 7.2 us, cut up 11.1; but 16 x
-  // 1 .. 1000, 32 / 8 heads of 128: 20.2 us cut up, 22.0 whole).
+  // At least 32 positions per warp (1 x 1000 positions, 6 fp32 heads of 64: 10.3 us, with 64 at least 13.4);
+  // whole parts in a block where the longest has up to 64 per warp (1 x 200: 7.4 us, cut up 11.1; but 16 x
+  // 1 .. 1000, 32 / 8 bf16 heads of 128: 17.3 us cut up, 19.9 whole).
   a.min_tiles = std::max(1, 32 / P::KT);
   a.whole_tiles = std::min(4, 64 / P::KT);
   a.box_rows = P::KT;

@@ -215,10 +215,10 @@ int rules_launch(cudaStream_t st, const RuleArgs& a, int rows, bool vec) {
 // arrived and store it.  The blocks of k_logit_rules wait for their ids, then for the touched logits,
 // with nothing else to do; here both lie in shared memory before they are wanted.  When a block comes to
 // a row of several slices it sorts the row's ids by slice once, so that each slice sees only its own (80 ->
-// 65 us for 256 rows x 128000 ids with 4000 known ids a row).  Measured there: 66 us, 4.0 TB/s, against 44 us
-// without any rule: sort, count, apply and mask of a slice are short steps between barriers, 4200 cycles
-// per 8000 ids where the memory would need 3000.  Slices as long as shared memory allows: 5120 ids and a
-// longer ring took 94 us.
+// 65 us for 256 rows x 128000 ids with 4000 known ids a row).  Measured there, with 300 biases and masks: 69 us,
+// 3.9 TB/s, against 44 us without any rule: sort, count, apply and mask of a slice follow one another between
+// barriers on the same warps, 4200 cycles per 8000 ids where the memory would need 3000.  Slices as long as
+// shared memory allows: 5120 ids and a longer ring took 94 us.
 constexpr int kMostIds = 8192, kRing = 3, kWorkers = 512;
 constexpr int kTokenRoom = 4096, kBiasRoom = 512;  // per slice; what is beyond is read from L2
 constexpr int kSorted = 64;                        // slices of a row up to which its ids are sorted
@@ -676,7 +676,7 @@ extern "C" int turt_logit_rules_apply(turt_ctx* ctx, const float* logits, size_t
   a.flags = ctx->flags;
   // every row of in and out starts equally far from a 16-byte boundary
   const bool vec = ((uintptr_t)logits & 15) == ((uintptr_t)out & 15) && (rows == 1 || ld % 4 == out_ld % 4);
-  // The pipeline where every SM gets several slices (256 x 128000: 66 us, one block per slice 100 us; but
+  // The pipeline where every SM gets several slices (256 x 128000: 69 us, one block per slice 100 us; but
   // 64 x 50001: 11.5 us, one block per slice 9.5 us); short slices where even those would leave SMs idle
   // (1 x 8192: 3.2 us, slices of 4096 4.0 us; 64 x 50001: 12.3 us, slices of 4096 9.5 us).
   const long enough = 4 * 148;
