@@ -142,3 +142,39 @@ def test_sequences_that_are_not_finite_among_others(eng, dtype, dim, heads, wind
     assert torch.isnan(out.view(len(lens), heads, dim)[bad][..., 1]).all()
     again, _ = attend(eng, c, q, heads, window=window)
     assert torch.equal(again[good], out[good])
+
+
+def test_more_tiles_than_32_bits_count(eng):
+    """One sequence of nearly 2^31 positions and 80 key heads, 5.4e9 tiles of 32 positions.  All pages but the last three
+    are one page whose scores lie 10^4 below, e^-10000 of the weight and 0 in fp32; the last three are others, so the
+    output is theirs alone."""
+    from turt_b200.runtime import make_paged_kv
+    kvh, dim, page = 80, 8, 4096
+    width = (1 << 31) // page - 1
+    g = torch.Generator().manual_seed(4)
+    k = torch.randn(4, kvh, page, dim, generator=g).bfloat16()
+    v = torch.randn(4, kvh, page, dim, generator=g).bfloat16()
+    q = torch.randn(1, kvh * dim, generator=g)
+    q[:, 0::dim] = math.sqrt(dim)
+    k[..., 0] = 0
+    k[0, ..., 0] = -10000
+    table = torch.zeros(1, width, dtype=torch.int32)
+    table[0, -3:] = torch.tensor([2, 1, 3])
+    n = width * page - 100
+    k_, v_, q_, t_ = k.cuda(), v.cuda(), q.cuda(), table.cuda()
+    lens = torch.tensor([n], dtype=torch.int32).cuda()
+    kv = make_paged_kv(k_.data_ptr(), v_.data_ptr(), t_.data_ptr(), lens.data_ptr(), "bf16", 4, page, kvh, dim, 1, width)
+    out = torch.full((1, kvh * dim), math.nan, device="cuda")
+    space = torch.zeros(eng.pagedAttentionWorkspace(kv, kvh), dtype=torch.uint8, device="cuda")
+    eng.pagedAttention(kv, q_.data_ptr(), kvh * dim, out.data_ptr(), kvh * dim, kvh, space.data_ptr(), space.numel())
+    eng.ctx.synchronize()
+    kk, vv = (x[[2, 1, 3]].transpose(1, 2).reshape(3 * page, kvh, dim)[:3 * page - 100].double() for x in (k, v))
+    qq = q.double().view(kvh, dim)
+    s = torch.einsum("nhd,hd->nh", kk, qq) / math.sqrt(dim)
+    p = torch.softmax(s, 0)
+    want = torch.einsum("nh,nhd->hd", p, vv).reshape(1, -1)
+    # expect()'s bound with the positions that have a weight
+    d = ((dim + 4) * 2.0 ** -23 / math.sqrt(dim) * torch.einsum("nhd,hd->nh", kk.abs(), qq.abs())).amax(0)
+    d = d + 8 * 2.0 ** -23 * (s.amax(0) - s.amin(0))
+    w = 2 * d + 2.0 ** -20 + 2 * (3 * page + 64) * 2.0 ** -23
+    close(out.cpu(), want, (w[:, None] * torch.einsum("nh,nhd->hd", p, vv.abs())).reshape(1, -1))

@@ -951,9 +951,9 @@ __global__ void __launch_bounds__(P::WARPS * 32, P::BLOCKS)
       x += places();
       at.s = seq_of<KT>(a, ++at.b);
     }
-    const uint32_t in = (uint32_t)(u - x), part = at.s.t1 - at.s.t0 + kPartCost;  // below 2^27 tiles times key heads
-    at.hc = (int)(in / part);
-    const uint32_t off = in - at.hc * part, tile = off > kPartCost ? off - kPartCost : 0;
+    const uint32_t part = at.s.t1 - at.s.t0 + kPartCost;
+    at.hc = (int)div64(u - x, part);  // (a long sequence times its key heads passes 32 bits)
+    const uint32_t off = (uint32_t)(u - x - (unsigned long long)at.hc * part), tile = off > kPartCost ? off - kPartCost : 0;
     at.t = at.s.t0 + tile;
     at.pos = u - off + kPartCost + tile;
     return u - off;
