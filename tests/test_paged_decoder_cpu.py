@@ -97,29 +97,29 @@ def test_a_forward_that_fails_keeps_no_buffer():
     assert g.engine.peak - sum(g.engine.live.values()) >= 2 * 30 * 30  # scores of 30 rows
 
 
-def test_no_position_beyond_what_is_reserved():
+def test_no_position_beyond_the_pages():
     """A step or prompt that a sequence has no pages for is refused before anything runs: it would go to another
-    sequence's page."""
+    sequence's page.  What its last page has room for is taken."""
     g = booked_gpt(2)
     dec = PagedDecoder(g, [18, 40], page_size=8)
     # table entries behind a sequence's pages name no page
     table = g.engine.uploads[dec.table].view("int32").reshape(2, 5)
     assert table.tolist() == [[0, 1, 2, -1, -1], [3, 4, 5, 6, 7]]
-    with pytest.raises(ValueError, match="19 positions, 18 are reserved"):
-        dec.prefill([[1] * 19, [2]])
+    with pytest.raises(ValueError, match="25 positions, its pages hold 24"):
+        dec.prefill([[1] * 25, [2]])
     for bad in ([[1]], [[1], []], [[1], [2], [3]]):
         with pytest.raises(ValueError):
             dec.prefill(bad)
-    dec.prefill([[1] * 17, [2]])
+    dec.prefill([[1] * 23, [2]])
     dec.step([1, 1])
     n = len(g.engine.calls)
-    with pytest.raises(ValueError, match="19 positions, 18 are reserved"):
+    with pytest.raises(ValueError, match="25 positions, its pages hold 24"):
         dec.step([1, 1])
     with pytest.raises(ValueError):
         dec.step([1])
-    assert len(g.engine.calls) == n and dec.lens.tolist() == [18, 2]
+    assert len(g.engine.calls) == n and dec.lens.tolist() == [24, 2]
     dec.step([None, 1])
-    assert dec.lens.tolist() == [18, 3]
+    assert dec.lens.tolist() == [24, 3]
 
 
 def test_a_step_that_fails_leaves_the_lengths():

@@ -242,7 +242,7 @@ class PagedDecoder:
             raise ValueError(f"{max(lengths)} positions exceed block size {c['blockSize']}")
         need = [-(-n // page_size) for n in lengths]
         self.n_pages, self.width = sum(need), max(need)
-        self.room = np.array(lengths, np.int64)
+        self.room = np.array(need, np.int64) * page_size
         table = np.full((self.batch, self.width), 0xFFFFFFFF, np.uint32)  # no page
         page = 0
         for b, n in enumerate(need):
@@ -384,7 +384,7 @@ class PagedDecoder:
 
     def _fits(self, lens) -> None:
         for i in np.flatnonzero(lens > self.room):
-            raise ValueError(f"sequence {i} would hold {lens[i]} positions, {self.room[i]} are reserved")
+            raise ValueError(f"sequence {i} would hold {lens[i]} positions, its pages hold {self.room[i]}")
 
     def prefill(self, prompts) -> int:
         if len(prompts) != self.batch or not all(len(p) for p in prompts):
